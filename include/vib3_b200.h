@@ -362,6 +362,56 @@ int vib3_launch_moe_grouped_int4(void* handle, const void* x, int x_dtype, int x
                                  float shared_weight, int pages_per_segment, int expert_lo, int expert_hi, float* out,
                                  int out_stride, int out_accumulate, int* status, void* stream);
 
+/* ── Latent attention: the cache, the attention over it and its per-head products ───────────────────────────── */
+/* A layer with latent attention keeps ONE row of 576 values per token for all heads: a latent of 512 values that is key and
+ * value at once, and 64 rotated position values that are key only.  The reference has scalar kernels for one token and a flat
+ * cache (cuda/src/kernels.cu:1570, :1624, :1679, :1709); these launchers take the tokens of a step and a paged cache.
+ * Strides are in ELEMENTS and multiples of 16 bytes, pointers 16-byte aligned (VIB3_ERR_ALIGN); the last dimension of every
+ * matrix is contiguous; dtypes are VIB3_X_F16 or VIB3_X_BF16, one for all 16-bit operands of a call.  n_tokens, batch or q_len 0:
+ * nothing is launched.  The launches are programmatic dependents that read nothing before their predecessor has finished.
+ * inv_freq: 32 doubles on the device, one per pair of position values; the angle position * inv_freq[i] is formed in 64 bits.
+ * pairs != 0: value 2 i turns with value 2 i + 1; 0: value i with value i + 32.  rope_scale multiplies the rotated values. */
+
+/* Append n_tokens rows to the cache: kv [n_tokens][576] (VIB3_X_*, kv_stride apart) holds the latents and the unrotated
+ * position values.  latent = kv[:512] / sqrt(mean of squares + eps) * norm_weight (norm_weight: 512 values of the cache's type;
+ * NULL: the latent as it is), position values rotated, both rounded once to the cache's type.  Row t goes to slot slots[t] =
+ * page * page_size + row of cache [num_pages][page_size][576]; a negative slot skips the token (padding), one beyond the cache
+ * skips it too and sets VIB3_STATUS_MISSING_PAGE in *status (may be NULL).  The slots of a call are distinct: with two tokens of one
+ * slot the row may hold parts of both.  Rows that no slot names are not touched. */
+int vib3_launch_latent_append_paged(const void* kv, int kv_dtype, long long kv_stride, const void* norm_weight_or_null, float eps,
+                                    const int* positions, const long long* slots, const double* inv_freq, float rope_scale, int pairs,
+                                    int n_tokens, void* cache, int cache_dtype, long long num_pages, int page_size,
+                                    long long page_stride, long long row_stride, int* status, void* stream);
+/* The heads' queries in the latent space: q [n_tokens][heads][nope + 64], w_uk [heads][nope][512] (rows contiguous, heads
+ * w_head_stride apart): out[t][h][:512] = q[t][h][:nope] . w_uk[h], out[t][h][512:] = q[t][h][nope:] rotated by positions[t].
+ * nope: a multiple of 16 up to 256; heads <= 128; n_tokens <= 262144. */
+int vib3_launch_latent_query(const void* q, long long q_token_stride, long long q_head_stride, const void* w_uk, long long w_head_stride,
+                             const int* positions, const double* inv_freq, float rope_scale, int pairs, void* out,
+                             long long out_token_stride, long long out_head_stride, int n_tokens, int heads, int nope, int dtype,
+                             void* stream);
+/* The heads' outputs: o [n_tokens][heads][512], w_uv [heads][value][512]: out[t][h][v] = o[t][h] . w_uv[h][v].  value: a multiple
+ * of 16 up to 256.  (w_uk and w_uv may be views of one matrix [heads][nope + value][512].) */
+int vib3_launch_latent_value(const void* o, long long o_token_stride, long long o_head_stride, const void* w_uv, long long w_head_stride,
+                             void* out, long long out_token_stride, long long out_head_stride, int n_tokens, int heads, int value,
+                             int dtype, void* stream);
+/* Attention of the q_len newest tokens of each of `batch` sequences over the paged cache, in the latent space.  q [batch *
+ * q_len][heads][576] (sequence b's tokens at rows b * q_len ..), seq_lens[b]: keys of sequence b with its new tokens; token j of
+ * q_len stands at position seq_lens[b] - q_len + j and sees the keys up to that position (none, if it is negative: out = 0, lse =
+ * -inf; a sequence with fewer new tokens has them last).  Key k of sequence b is row k % page_size of page page_table[b *
+ * table_stride + k / page_size].  out [batch * q_len][heads][512] = softmax(scale * q . keys) . keys[:, :512]; lse (may be NULL): fp32
+ * [batch * q_len][heads], the natural logarithm of the softmax's denominator, scale included.  A key whose page number is not in
+ * [0, num_pages), or whose table entry lies beyond max_pages_per_seq, is left out and VIB3_STATUS_MISSING_PAGE is set.  Rows of the cache behind a
+ * sequence's length may hold anything; those within it are read by every token of the call that shares a tile with them and have to be
+ * finite.  page_size: a multiple of 8; heads <= 128; batch * q_len <= 1048576.  workspace: at least
+ * vib3_latent_attention_workspace_bytes(), contents irrelevant; calls sharing a workspace must not overlap. */
+size_t vib3_latent_attention_workspace_bytes(void);
+int vib3_launch_latent_attention_paged(const void* q, long long q_token_stride, long long q_head_stride, const void* cache,
+                                       long long num_pages, int page_size, long long page_stride, long long row_stride,
+                                       const int* page_table, int table_stride, int max_pages_per_seq, const int* seq_lens, int batch,
+                                       int q_len, int heads, float scale, int dtype, void* out, long long out_token_stride,
+                                       long long out_head_stride, float* lse_or_null, void* workspace, size_t workspace_bytes,
+                                       int* status, void* stream);
+
 /* Library options.  key 0: use the bulk-copy staged MoE kernels where the shape allows (default 1);
  * 0 forces the direct-load kernels.  key 1: launch the staged kernels with programmatic dependent
  * launch so that their prologue overlaps the previous kernel's tail (default 1).  key 2:

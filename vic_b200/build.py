@@ -19,6 +19,8 @@ SOURCES = [
     "moe_grouped.cu",
     "ep_peer.cu",
     "router.cu",
+    "latent_ops.cu",
+    "latent_attention.cu",
     "host/page_pool.cpp",
     "host/vib3_file.cpp",
 ]

@@ -34,7 +34,7 @@ class ResolvedPage(C.Structure):
                 ("row_start", C.c_uint16), ("row_count", C.c_uint16)]
 
 
-_vp, _i, _f = C.c_void_p, C.c_int, C.c_float
+_vp, _i, _f, _ll = C.c_void_p, C.c_int, C.c_float, C.c_longlong
 
 # every symbol include/vib3_b200.h declares, with its argument types
 SIGNATURES = {
@@ -90,6 +90,12 @@ SIGNATURES = {
                                            _i, _vp, _vp]),
     "vib3_launch_rms_norm_f32": (_i, [_vp, _vp, _vp, _i, _f, _vp]),
     "vib3_launch_residual_rms_norm": (_i, [_vp, _i, _vp, _i, _i, _vp, _i, _vp, _f, _i, _vp, _i, _i, _i, _i, _vp]),
+    "vib3_launch_latent_append_paged": (_i, [_vp, _i, _ll, _vp, _f, _vp, _vp, _vp, _f, _i, _i, _vp, _i, _ll, _i, _ll, _ll, _vp, _vp]),
+    "vib3_launch_latent_query": (_i, [_vp, _ll, _ll, _vp, _ll, _vp, _vp, _f, _i, _vp, _ll, _ll, _i, _i, _i, _i, _vp]),
+    "vib3_launch_latent_value": (_i, [_vp, _ll, _ll, _vp, _ll, _vp, _ll, _ll, _i, _i, _i, _i, _vp]),
+    "vib3_latent_attention_workspace_bytes": (C.c_size_t, []),
+    "vib3_launch_latent_attention_paged": (_i, [_vp, _ll, _ll, _vp, _ll, _i, _ll, _ll, _vp, _i, _i, _vp, _i, _i, _i, _f, _i, _vp, _ll,
+                                                _ll, _vp, _vp, C.c_size_t, _vp, _vp]),
     "vib3_config_set": (_i, [_i, _i]),
     "vib3_pool_create": (_vp, [_vp, C.c_size_t, C.c_uint64]),
     "vib3_pool_destroy": (None, [_vp]),
