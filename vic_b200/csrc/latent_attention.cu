@@ -30,9 +30,9 @@ constexpr int kChunkBytes = 64 * 128;                     // 64 rows of 64 value
 constexpr int kChunks = kLatentRow / 64;                  // 9: eight of the latent, one of position values
 constexpr int kTileBytes = kChunks * kChunkBytes;
 constexpr int kGroups = 5;                                // pieces of a tile: chunk pairs 0..3, the position chunk
-constexpr int kQOff = 0, kKvOff = kTileBytes, kPOff = 3 * kTileBytes, kMiscOff = kPOff + kChunkBytes;
-constexpr int kAttThreads = 256;                          // copies, MMAs, two warps for Q, four for the softmax and the results
-constexpr int kSoftmaxThreads = 128;
+constexpr int kQOff = 0, kKvOff = kTileBytes, kPOff = 8 * kChunkBytes /* in a tile */, kMiscOff = 3 * kTileBytes;
+constexpr int kAttThreads = 384;                          // copies, MMAs, two warps for Q, eight for the softmax and the results
+constexpr int kSoftmaxThreads = 256;
 constexpr int kTmemCols = 512, kSCol = 256;               // O^T: 4 x 64 columns, S: 2 x 64
 // The reference m of a row follows its maximum only when that has grown by more than 2^8: exp(s - m) then stays below 256, the
 // 16-bit weights keep their relative precision, and the accumulator is rescaled a few times per sequence instead of per tile.
@@ -117,10 +117,11 @@ struct Walk {
 };
 
 struct AttShared {
-    uint64_t kv_full[2][kGroups], kv_empty[2][kGroups];
-    uint64_t s_full[2], p_full, pv_done, q_full, q_empty, drain;
+    uint64_t kv_full[2], kv_empty[2][kGroups];
+    uint64_t s_full[2], p_full[2], pv_done[2], q_full, q_empty, drain;
     unsigned long long mask[2];            // keys of the tile that count
-    alignas(16) float factor[2][kTileRows];
+    alignas(16) float factor[kTileRows];
+    float team[2][kTileRows];              // what the two softmax teams have of a row: maximum, sum
     alignas(16) float inv[kTileRows];
     Plan plan;
     long long warp_sum[kAttThreads / 32];
@@ -148,8 +149,20 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, unsigned parity) {
                      : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
     return ok != 0;
 }
+// One look, without waiting; the warp's lanes agree.
+__device__ __forceinline__ bool bar_test(uint64_t* bar, unsigned parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return __all_sync(0xffffffffu, ok != 0);
+}
+constexpr unsigned kIdleLimit = 1u << 26;   // looks without progress (each some 50 cycles: about two seconds)
 // The same for a whole warp, whose lanes have to agree (they meet again in warp-wide instructions).
 __device__ __forceinline__ bool bar_wait_warp(uint64_t* bar, unsigned parity) { return __all_sync(0xffffffffu, bar_wait(bar, parity)); }
+// 16 bytes global -> shared, zeros where !live
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
 // One lane of the warp, the same one every time: behind elect.sync MMAs and tensor copies issue back to back.
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -163,9 +176,19 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+// Shared-memory operands with 128-byte swizzle.  K-major: rows of 128 bytes, eight of them 1024 bytes.  MN-major: 64 values
+// contiguous per key, eight keys 1024 bytes, the next 64 values a chunk further.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | ((uint32_t)(kChunkBytes >> 4) << 16); }
+// A value that is the same in all lanes, told to the compiler: an MMA takes its operands from uniform registers, and with
+// operands that it had to move there one by one an MMA of this kernel cost 85 cycles instead of the pipe's 32 or 48.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+// Operands by the low words of their descriptors (the address); the high words are constants.
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+                 ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kDescHigh) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -186,25 +209,17 @@ __device__ __forceinline__ bool softmax_any(bool v) {
     return r != 0;
 }
 
-// Shared-memory operands with 128-byte swizzle.  K-major: rows of 128 bytes, eight of them 1024 bytes.  MN-major: 64 values
-// contiguous per key, eight keys 1024 bytes, the next 64 values a chunk further.
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(kChunkBytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)2 << 61);
-}
 template <typename T> constexpr uint32_t kFormat = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
 template <typename T> constexpr uint32_t kIdescS = (1u << 4) | (kFormat<T> << 7) | (kFormat<T> << 10) | (64u / 8 << 17) | (64u / 16 << 24);
 template <typename T> constexpr uint32_t kIdescO = (1u << 4) | (kFormat<T> << 7) | (kFormat<T> << 10) | (1u << 15) | (64u / 8 << 17) | (128u / 16 << 24);
 
-__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t* r) {
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+// 16 lanes x 32 columns: thread t has columns 8 x + 2 (t & 3) + {0, 1} of lane t / 4 (registers 4 x, 4 x + 1) and of lane t / 4 + 8.
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr) : "memory");
 }
-
+// 32 lanes x 32 columns, a lane per thread.
 __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t* r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
@@ -216,78 +231,79 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t* r)
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
 
-// This CTA's place on its lane's line of tiles.  All threads.
+// This CTA's place on its lane's line of tiles.  All threads.  Up to kAttThreads items are read once and stay in registers.
 __device__ __forceinline__ void make_plan(const AttentionArgs& a, AttShared& sh) {
+    constexpr int kWarps = kAttThreads / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int row_lane = blockIdx.x % a.lanes, share = blockIdx.x / a.lanes, items = item_count(a);
+    const int row_lane = a.lanes == 1 ? 0 : blockIdx.x % a.lanes, share = a.lanes == 1 ? blockIdx.x : blockIdx.x / a.lanes, items = item_count(a);
+    const int most = a.lanes == 1 ? gridDim.x : gridDim.x / a.lanes;
     Piece p;
-    auto block_sum = [&](long long v) {
-#pragma unroll
-        for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-        __syncthreads();
-        if (lane == 0) sh.warp_sum[warp] = v;
-        __syncthreads();
-        v = 0;
-#pragma unroll
-        for (int w = 0; w < kAttThreads / 32; ++w) v += sh.warp_sum[w];
-        return v;
-    };
-    long long mine = 0;
-    for (int i = tid; i < items; i += kAttThreads) {
+    auto tiles_of = [&](int i) {
+        if (i >= items) return 0;
         item_of(a, row_lane, i, p);
-        mine += p.tiles;
-    }
-    const long long total = block_sum(mine);
-    const int most = gridDim.x / a.lanes;
+        return p.tiles;
+    };
+    // inclusive sum over the block's threads; `sum` receives the total
+    auto block_scan = [&](long long v, long long& sum) {
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+            const long long o = __shfl_up_sync(0xffffffffu, v, m);
+            if (lane >= m) v += o;
+        }
+        __syncthreads();
+        if (lane == 31) sh.warp_sum[warp] = v;
+        __syncthreads();
+        sum = 0;
+        long long before = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w == warp) before = sum;
+            sum += sh.warp_sum[w];
+        }
+        return before + v;
+    };
+    const int first_tiles = tiles_of(tid);
+    long long mine = first_tiles, chunk, total;
+    for (int i = tid + kAttThreads; i < items; i += kAttThreads) mine += tiles_of(i);
+    long long incl = block_scan(mine, total);
     const int shares = (int)max(1ll, min((long long)most, (total + a.min_tiles - 1) / a.min_tiles));
-    const long long begin = share < shares ? total * share / shares : total, end = share < shares ? total * (share + 1) / shares : total;
+    const bool idle = share >= shares;
+    // (a 64-bit division is a subroutine of some hundred instructions)
+    auto cut = [&](int k) {
+        return total <= 0x7fffffff / kMaxGrid ? (long long)((unsigned)total * (unsigned)k / (unsigned)shares) : total * k / shares;
+    };
+    const long long begin = idle ? total : cut(share), end = idle ? total : cut(share + 1);
     if (tid == 0) {
         sh.plan.begin = begin; sh.plan.end = end; sh.plan.total = total;
-        sh.plan.item = items; sh.plan.prefix = total; sh.plan.lane = row_lane; sh.plan.share = share; sh.plan.shares = shares;
+        sh.plan.lane = row_lane; sh.plan.share = share; sh.plan.shares = shares;
+        if (idle) {
+            sh.plan.item = items;
+            sh.plan.prefix = total;
+        }
     }
-    if (share >= shares) {
-        __syncthreads();
-        return;
-    }
+    if (idle) return;
     // the first item that begins at `begin` or reaches beyond it
     long long base = 0;
     for (int i0 = 0; i0 < items; i0 += kAttThreads) {
-        const int i = i0 + tid;
-        long long tiles = 0;
-        if (i < items) {
-            item_of(a, row_lane, i, p);
-            tiles = p.tiles;
+        const int i = i0 + tid, tiles = i0 == 0 ? first_tiles : tiles_of(i);
+        if (items > kAttThreads) incl = block_scan(tiles, chunk);
+        else chunk = total;
+        const long long pre = base + incl - tiles;
+        // of those that qualify the first one: nothing before it begins at `begin`, and what comes before does not reach beyond
+        if (i < items && pre <= begin && (pre == begin || pre + tiles > begin)) {
+            bool first = true;
+            if (pre == begin && i > 0) {   // an item before this one with the same beginning (no tiles) comes first
+                item_of(a, row_lane, i - 1, p);
+                first = p.tiles > 0;
+            }
+            if (first) {
+                sh.plan.item = i;
+                sh.plan.prefix = pre;
+            }
         }
-        long long incl = tiles;
-#pragma unroll
-        for (int m = 1; m < 32; m <<= 1) {
-            const long long o = __shfl_up_sync(0xffffffffu, incl, m);
-            if (lane >= m) incl += o;
-        }
-        __syncthreads();
-        if (lane == 31) sh.warp_sum[warp] = incl;
-        __syncthreads();
-        long long before = base;
-        for (int w = 0; w < warp; ++w) before += sh.warp_sum[w];
-        const long long pre = before + incl - tiles;
-        const bool mineIs = i < items && (pre == begin || pre + tiles > begin);
-        // (one thread: the item before it does not qualify)
-        const unsigned hits = __ballot_sync(0xffffffffu, mineIs);
-        bool first = mineIs && (hits & ((1u << lane) - 1)) == 0;
-        if (first && lane == 0 && i > 0) {   // the previous item is another warp's (or chunk's)
-            Piece prev;
-            item_of(a, row_lane, i - 1, prev);
-            const long long ppre = pre - prev.tiles;
-            first = !(ppre == begin || pre > begin);
-        }
-        if (first) {
-            sh.plan.item = i;
-            sh.plan.prefix = pre;
-        }
-        for (int w = 0; w < kAttThreads / 32; ++w) base += sh.warp_sum[w];
+        base += chunk;
         if (base > begin) break;
     }
-    __syncthreads();
 }
 
 template <typename T>
@@ -298,14 +314,12 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     if (tid == 0) {
         for (int s = 0; s < 2; ++s) {
-            for (int g = 0; g < kGroups; ++g) {
-                bar_init(&sh.kv_full[s][g], 1);
-                bar_init(&sh.kv_empty[s][g], 1);
-            }
+            bar_init(&sh.kv_full[s], 1);
+            for (int g = 0; g < kGroups; ++g) bar_init(&sh.kv_empty[s][g], 1);
             bar_init(&sh.s_full[s], 1);
+            bar_init(&sh.p_full[s], kSoftmaxThreads);
+            bar_init(&sh.pv_done[s], 1);
         }
-        bar_init(&sh.p_full, kSoftmaxThreads);
-        bar_init(&sh.pv_done, 1);
         bar_init(&sh.q_full, 64);
         bar_init(&sh.q_empty, 1);
         bar_init(&sh.drain, 1);
@@ -321,7 +335,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh.tmem;
+    const uint32_t tmem = uniform(sh.tmem);
     const Plan& plan = sh.plan;
     const int rows_all = a.q_len * a.heads;
     Walk walk(a, plan);
@@ -331,7 +345,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
     if (warp == 0) {
         // ── copies: the tiles of C, in boxes of box_rows rows that lie in one page ──
         const int R = a.box_rows, nb = kTileKeys / R, per_load = 32 / nb;
-        int it = 0, issued = kGroups;   // pieces of the newest tile that were requested
+        int it = 0;
         while (ok && walk.next(p, false)) {
             int page_of = 0, loaded = -1;
             for (int t = p.t0; ok && t < p.t1; ++t, ++it) {
@@ -355,83 +369,102 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
 #pragma unroll
                 for (int g = 0; g < kGroups; ++g) {
                     if (use > 0 && !bar_wait_warp(&sh.kv_empty[s][g], (use - 1) & 1)) {
+                        // the tile's remaining bytes will not come: what was requested is waited for below, this tile cannot be
                         ok = false;
-                        issued = g;
                         break;
                     }
-                    if (lane == 0) {
-                        if (g == 0) sh.mask[s] = m;
-                        bar_expect(&sh.kv_full[s][g], g < 4 ? 2 * kChunkBytes : kChunkBytes);
+                    if (g == 0) {
+                        if (lane == 0) {
+                            sh.mask[s] = m;
+                            bar_expect(&sh.kv_full[s], kTileBytes);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                     if (mine) {
-                        tma_load_3d(dst + 2 * g * kChunkBytes, &map, 2 * g * 64, y, z, &sh.kv_full[s][g]);
-                        if (g < 4) tma_load_3d(dst + (2 * g + 1) * kChunkBytes, &map, (2 * g + 1) * 64, y, z, &sh.kv_full[s][g]);
+                        tma_load_3d(dst + 2 * g * kChunkBytes, &map, 2 * g * 64, y, z, &sh.kv_full[s]);
+                        if (g < 4) tma_load_3d(dst + (2 * g + 1) * kChunkBytes, &map, (2 * g + 1) * 64, y, z, &sh.kv_full[s]);
                     }
                     __syncwarp();
                 }
             }
         }
-        // nothing is owed to this CTA's memory when it leaves: neither the releases of the last tiles nor, after a wait that
-        // ran out, copies in flight
+        // Nothing is owed to this CTA's memory when it leaves: the releases of the last tiles arrive, or, after a wait that ran out,
+        // the copies in flight do (the newest tile's barrier may lack bytes that were never requested: that wait gives up).
         for (int n = max(it - 2, 0); n < it; ++n)
-            for (int g = 0; g < (n == it - 1 ? issued : kGroups); ++g)
+            for (int g = 0; g < kGroups; ++g)
                 if (!ok || !bar_wait_warp(&sh.kv_empty[n & 1][g], (n >> 1) & 1)) {
                     ok = false;
-                    bar_wait_warp(&sh.kv_full[n & 1][g], (n >> 1) & 1);
+                    bar_wait_warp(&sh.kv_full[n & 1], (n >> 1) & 1);
+                    break;
                 }
     } else if (warp == 1) {
         // ── MMAs ──
-        int it = 0, pieces = 0;
-        const uint32_t q = base + kQOff, pb = base + kPOff;
-        auto scores = [&](int n, bool last) {      // S of tile n
-            const int s = n & 1;
-            const uint32_t c = base + kKvOff + s * kTileBytes, d = tmem + kSCol + 64 * s;
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-                if (!bar_wait_warp(&sh.kv_full[s][g], (n >> 1) & 1)) return false;
+        // Two walks over the same tiles, S at most two tiles ahead of O (its two buffers).  Whatever has its operands goes next, O
+        // first, since only O gives shared memory back: with S(i + 1) always before O(i), O waited for the load of tile i + 1,
+        // which waits for the room of tile i - 1, and a tile took 4100 cycles.
+        Walk walk_o(a, plan);
+        Piece po;
+        bool more_s = ok && walk.next(p, false), more_o = ok && walk_o.next(po, false);
+        int ns = 0, ts = p.t0, q_pieces = 0;              // next S: tile count, tile of the item, pieces whose Q was read
+        int no = 0, to = po.t0;                           // next O
+        bool q_ready = false;
+        unsigned idle = 0;
+        while (more_o) {
+            if (no < ns && bar_test(&sh.p_full[no & 1], (no >> 1) & 1)) {
                 tc_fence_after();
-                if (elect_one()) {
-#pragma unroll
-                    for (int k = 0; k < (g < 4 ? 8 : 4); ++k) {
-                        const uint32_t off = (2 * g + (k >> 2)) * kChunkBytes + (k & 3) * 32;
-                        umma_ss(d, desc_k(q + off), desc_k(c + off), kIdescS<T>, (uint32_t)(g + k > 0));
-                    }
-                }
-                __syncwarp();
-            }
-            if (elect_one()) {
-                umma_commit(&sh.s_full[s]);
-                umma_commit(&sh.kv_empty[s][4]);
-                if (last) umma_commit(&sh.q_empty);
-            }
-            __syncwarp();
-            return true;
-        };
-        while (ok && walk.next(p, false)) {
-            const int n = p.t1 - p.t0;
-            ok = bar_wait_warp(&sh.q_full, pieces & 1);
-            tc_fence_after();
-            ok = ok && scores(it, n == 1);
-            for (int i = 0; ok && i < n; ++i, ++it) {
-                if (i + 1 < n) ok = scores(it + 1, i + 2 == n);
-                ok = ok && bar_wait_warp(&sh.p_full, it & 1);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t c = base + kKvOff + (it & 1) * kTileBytes;
+                const int st = (int)uniform((uint32_t)no & 1);
+                const uint32_t c = uniform(base + kKvOff + st * kTileBytes), v = desc_mn(c), pk = desc_k(c + kPOff), acc = uniform(to > po.t0);
                 if (elect_one()) {
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            umma_ss(tmem + 64 * g, desc_mn(c + 2 * g * kChunkBytes + k * 2048), desc_k(pb + k * 32), kIdescO<T>, (uint32_t)(i + k > 0));
-                        umma_commit(&sh.kv_empty[it & 1][g]);
+                            umma_ss(tmem + 64 * g, v + (2 * g * kChunkBytes + k * 2048) / 16, pk + k * 2, kIdescO<T>, k > 0 ? 1u : acc);
+                        umma_commit(&sh.kv_empty[st][g]);
                     }
-                    umma_commit(&sh.pv_done);
+                    umma_commit(&sh.kv_empty[st][kGroups - 1]);
+                    umma_commit(&sh.pv_done[st]);
                 }
                 __syncwarp();
+                ++no;
+                if (++to == po.t1) {
+                    more_o = walk_o.next(po, false);
+                    to = po.t0;
+                }
+                idle = 0;
+                continue;
             }
-            ++pieces;
+            if (more_s && ns < no + 2) {
+                if (!q_ready && bar_test(&sh.q_full, q_pieces & 1)) q_ready = true;
+                if (q_ready && bar_test(&sh.kv_full[ns & 1], (ns >> 1) & 1)) {
+                    tc_fence_after();
+                    const bool piece_end = ts + 1 == p.t1;
+                    const int st = (int)uniform((uint32_t)ns & 1);
+                    const uint32_t d = uniform(tmem + kSCol + 64 * st), qd = uniform(desc_k(base + kQOff)), cd = uniform(desc_k(base + kKvOff + st * kTileBytes));
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < 4 * kChunks; ++k)
+                            umma_ss(d, qd + (k >> 2) * kChunkBytes / 16 + (k & 3) * 2, cd + (k >> 2) * kChunkBytes / 16 + (k & 3) * 2, kIdescS<T>, k > 0);
+                        umma_commit(&sh.s_full[st]);
+                        if (piece_end) umma_commit(&sh.q_empty);
+                    }
+                    __syncwarp();
+                    ++ns;
+                    ++ts;
+                    if (piece_end) {
+                        q_ready = false;
+                        ++q_pieces;
+                        more_s = walk.next(p, false);
+                        ts = p.t0;
+                    }
+                    idle = 0;
+                    continue;
+                }
+            }
+            if (++idle > kIdleLimit) {
+                ok = false;
+                break;
+            }
         }
         if (!ok) {   // the MMAs that were issued have to be through before the tensor memory is freed
             if (elect_one()) umma_commit(&sh.drain);
@@ -440,20 +473,25 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
         }
     } else if (warp < 4) {
         // ── Q of a piece: 64 rows, zeros behind the last one ──
-        const int ltid = tid - 64;
         int pieces = 0;
         while (ok && walk.next(p, false)) {
-            if (pieces > 0) ok = bar_wait(&sh.q_empty, (pieces - 1) & 1);
+            if (pieces > 0) ok = bar_wait_warp(&sh.q_empty, (pieces - 1) & 1);
             if (!ok) break;
-            const T* q = (const T*)a.q + (long long)p.b * a.q_len * a.q_token;
-#pragma unroll 4
-            for (int i = ltid; i < kTileRows * (kLatentRow / 8); i += 64) {
-                const int r = i / (kLatentRow / 8), c = i - r * (kLatentRow / 8), row = p.rb * kTileRows + r;
-                const bool live = row < rows_all;
-                const int j = live ? row / a.heads : 0, h = live ? row - j * a.heads : 0;
-                const uint32_t dst = base + kQOff + (c >> 3) * kChunkBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(q + j * a.q_token + h * a.q_head + c * 8), "r"(live ? 16 : 0)
-                             : "memory");
+            const long long token0 = (long long)p.b * a.q_len;
+            // A warp takes every second row; lane i works out the address of its i-th (a division per 16 bytes: 8 us per piece).
+            const int row = p.rb * kTileRows + 2 * lane + (warp & 1), j = row / a.heads, h = row - j * a.heads;
+            const long long at = row < rows_all ? (token0 + j) * a.q_token + h * a.q_head : -1;
+            const uint32_t piece = (uint32_t)(lane & 7), chunk = base + kQOff + (lane >> 3) * kChunkBytes;
+#pragma unroll 8
+            for (int i = 0; i < kTileRows / 2; ++i) {
+                const long long off = __shfl_sync(0xffffffffu, at, i);
+                const bool live = off >= 0;
+                const T* src = (const T*)a.q + (live ? off : 0) + lane * 8;
+                const int r = 2 * i + (warp & 1);
+                const uint32_t dst = chunk + r * 128 + ((piece ^ (r & 7)) << 4);
+                cp_async16(dst, src, live);
+                cp_async16(dst + 4 * kChunkBytes, src + 256, live);
+                if (lane < 8) cp_async16(dst + 8 * kChunkBytes, src + 512, live);
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             proxy_fence();
@@ -463,8 +501,9 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
         if (ok && pieces > 0) ok = bar_wait(&sh.q_empty, (pieces - 1) & 1);
     } else {
         // ── softmax and results ──
-        // (a thread whose wait ran out goes on to the next common barrier, where all of them leave together)
-        const int w = warp & 3, r0 = 16 * w + (lane >> 2), r1 = r0 + 8, c0 = 2 * (lane & 3);
+        // Two teams of four warps, 32 keys each; warp w of a team has rows 16 w .. (their lanes in tensor memory), a thread two rows
+        // and eight keys of each.  (A thread whose wait ran out goes on to the next common barrier, where all of them leave.)
+        const int team = (warp - 4) >> 2, w = warp & 3, r0 = 16 * w + (lane >> 2), r1 = r0 + 8, c0 = 32 * team + 2 * (lane & 3);
         const uint32_t quarter = (uint32_t)(32 * w) << 16;
         const int stid = tid - 128;
         if (stid == 0) a.owner[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -475,7 +514,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
             if (stid == 0 && len > a.max_pages * a.page_size && a.status) atomicOr(a.status, kStatusBadPage);
             if (p.tiles == 0) {      // no row of the block sees a key
                 const int n = min(kTileRows, rows_all - p.rb * kTileRows);
-                for (int r = w; r < n; r += 4) {
+                for (int r = warp - 4; r < n; r += 8) {
                     const int row = p.rb * kTileRows + r, j = row / a.heads, h = row - j * a.heads;
                     uint4* o = reinterpret_cast<uint4*>((T*)a.out + (token0 + j) * a.out_token + h * a.out_head);
                     o[lane] = o[lane + 32] = make_uint4(0, 0, 0, 0);
@@ -489,22 +528,24 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
             float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
             for (int t = p.t0; t < p.t1; ++t, ++it) {
                 const int s = it & 1, key0 = t * kTileKeys;
-                ok = ok && bar_wait(&sh.kv_full[s][0], (it >> 1) & 1) && bar_wait(&sh.s_full[s], (it >> 1) & 1);
+                const unsigned parity = (unsigned)(it >> 1) & 1;
+                // (the tile two before is through when this one's scores are; seen here, its phase cannot be taken for another)
+                ok = ok && (it < 2 || bar_wait(&sh.pv_done[s], parity ^ 1)) && bar_wait(&sh.kv_full[s], parity) && bar_wait(&sh.s_full[s], parity);
                 __syncwarp();
                 const unsigned long long mask = sh.mask[s];
                 tc_fence_after();
-                uint32_t raw[32];
-                tmem_ld_16x64(tmem + kSCol + 64 * s + quarter, raw);
+                uint32_t raw[16];
+                tmem_ld_16x32(tmem + kSCol + 64 * s + 32 * team + quarter, raw);
                 tmem_ld_wait();
-                float v[32];
+                float v[16];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]) * a.scale_log2;
+                for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(raw[i]) * a.scale_log2;
                 if (mask != ~0ull || key0 + kTileKeys > seen_all) {
                     // (values in masked places may be anything: they are replaced, not multiplied)
                     const unsigned long long k0 = seen0 - key0 >= 64 ? mask : seen0 > key0 ? mask & ((1ull << (seen0 - key0)) - 1) : 0ull;
                     const unsigned long long k1 = seen1 - key0 >= 64 ? mask : seen1 > key0 ? mask & ((1ull << (seen1 - key0)) - 1) : 0ull;
 #pragma unroll
-                    for (int x = 0; x < 8; ++x)
+                    for (int x = 0; x < 4; ++x)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             if (!(k0 >> (8 * x + c0 + e) & 1)) v[4 * x + e] = -INFINITY;
@@ -513,76 +554,75 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
                 }
                 float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
+                for (int x = 0; x < 4; ++x) {
                     x0 = fmaxf(x0, fmaxf(v[4 * x], v[4 * x + 1]));
                     x1 = fmaxf(x1, fmaxf(v[4 * x + 2], v[4 * x + 3]));
                 }
+                if (softmax_any(x0 > m0 + kLazy || x1 > m1 + kLazy || !ok)) {
+                    // a reference moves: the rows' maxima over both teams, then O's rows times exp2(old - new)
+                    ok = !softmax_any(!ok);
+                    if (!ok) break;
 #pragma unroll
-                for (int x = 1; x < 4; x <<= 1) {
-                    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, x));
-                    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, x));
-                }
-                float f0 = 1.f, f1 = 1.f;
-                if (x0 > m0 + kLazy) {
-                    f0 = m0 == -INFINITY ? 1.f : ex2(m0 - x0);
-                    m0 = x0;
-                    l0 *= f0;
-                }
-                if (x1 > m1 + kLazy) {
-                    f1 = m1 == -INFINITY ? 1.f : ex2(m1 - x1);
-                    m1 = x1;
-                    l1 *= f1;
-                }
-                if ((lane & 3) == 0) {
-                    sh.factor[s][r0] = f0;
-                    sh.factor[s][r1] = f1;
-                }
-                const bool rescale = softmax_any(f0 != 1.f || f1 != 1.f || !ok);
-                if (rescale && softmax_any(!ok)) {
-                    ok = false;
-                    break;
+                    for (int x = 1; x < 4; x <<= 1) {
+                        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, x));
+                        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, x));
+                    }
+                    if ((lane & 3) == 0) {
+                        sh.team[team][r0] = x0;
+                        sh.team[team][r1] = x1;
+                    }
+                    softmax_sync();
+                    x0 = fmaxf(x0, sh.team[team ^ 1][r0]);
+                    x1 = fmaxf(x1, sh.team[team ^ 1][r1]);
+                    float f0 = 1.f, f1 = 1.f;
+                    if (x0 > m0 + kLazy) {
+                        f0 = m0 == -INFINITY ? 1.f : ex2(m0 - x0);
+                        m0 = x0;
+                        l0 *= f0;
+                    }
+                    if (x1 > m1 + kLazy) {
+                        f1 = m1 == -INFINITY ? 1.f : ex2(m1 - x1);
+                        m1 = x1;
+                        l1 *= f1;
+                    }
+                    if (team == 0 && (lane & 3) == 0) {
+                        sh.factor[r0] = f0;
+                        sh.factor[r1] = f1;
+                    }
+                    softmax_sync();
+                    if (t > p.t0) {
+                        ok = bar_wait(&sh.pv_done[s ^ 1], (unsigned)((it - 1) >> 1) & 1);
+                        __syncwarp();
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int x = 4 * team; x < 4 * team + 4; ++x) {
+                            uint32_t o[32];
+                            tmem_ld_32x32(tmem + 32 * x + quarter, o);
+                            tmem_ld_wait();
+                            const float4* f = reinterpret_cast<const float4*>(&sh.factor[32 * (x & 1)]);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float4 y = f[i];
+                                o[4 * i] = __float_as_uint(__uint_as_float(o[4 * i]) * y.x);
+                                o[4 * i + 1] = __float_as_uint(__uint_as_float(o[4 * i + 1]) * y.y);
+                                o[4 * i + 2] = __float_as_uint(__uint_as_float(o[4 * i + 2]) * y.z);
+                                o[4 * i + 3] = __float_as_uint(__uint_as_float(o[4 * i + 3]) * y.w);
+                            }
+                            tmem_st_32x32(tmem + 32 * x + quarter, o);
+                        }
+                        tmem_st_wait();
+                    }
                 }
                 const float n0 = m0 == -INFINITY ? 0.f : m0, n1 = m1 == -INFINITY ? 0.f : m1;
-                float s0 = 0.f, s1 = 0.f;
+                // P takes the place of the tile's position values, which no product reads again
+                unsigned char* pr = smem + kKvOff + s * kTileBytes + kPOff + 4 * (lane & 3);
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    v[4 * x] = ex2(v[4 * x] - n0);
-                    v[4 * x + 1] = ex2(v[4 * x + 1] - n0);
-                    v[4 * x + 2] = ex2(v[4 * x + 2] - n1);
-                    v[4 * x + 3] = ex2(v[4 * x + 3] - n1);
-                    s0 += v[4 * x] + v[4 * x + 1];
-                    s1 += v[4 * x + 2] + v[4 * x + 3];
-                }
-                l0 += s0;
-                l1 += s1;
-                // P and O belong to the product of the tile before until that is through
-                if (it > 0) ok = bar_wait(&sh.pv_done, (it - 1) & 1);
-                __syncwarp();
-                if (rescale && t > p.t0) {
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int x = 0; x < 8; ++x) {
-                        uint32_t o[32];
-                        tmem_ld_32x32(tmem + 32 * x + quarter, o);
-                        tmem_ld_wait();
-                        const float4* f = reinterpret_cast<const float4*>(&sh.factor[s][32 * (x & 1)]);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float4 y = f[i];
-                            o[4 * i] = __float_as_uint(__uint_as_float(o[4 * i]) * y.x);
-                            o[4 * i + 1] = __float_as_uint(__uint_as_float(o[4 * i + 1]) * y.y);
-                            o[4 * i + 2] = __float_as_uint(__uint_as_float(o[4 * i + 2]) * y.z);
-                            o[4 * i + 3] = __float_as_uint(__uint_as_float(o[4 * i + 3]) * y.w);
-                        }
-                        tmem_st_32x32(tmem + 32 * x + quarter, o);
-                    }
-                    tmem_st_wait();
-                }
-                unsigned char* pr = smem + kPOff;
-#pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    *reinterpret_cast<uint32_t*>(pr + r0 * 128 + ((x ^ (r0 & 7)) << 4) + 2 * c0) = pack2<T>(v[4 * x], v[4 * x + 1]);
-                    *reinterpret_cast<uint32_t*>(pr + r1 * 128 + ((x ^ (r1 & 7)) << 4) + 2 * c0) = pack2<T>(v[4 * x + 2], v[4 * x + 3]);
+                for (int x = 0; x < 4; ++x) {
+                    const float e0 = ex2(v[4 * x] - n0), e1 = ex2(v[4 * x + 1] - n0), e2 = ex2(v[4 * x + 2] - n1), e3 = ex2(v[4 * x + 3] - n1);
+                    *reinterpret_cast<uint32_t*>(pr + r0 * 128 + (((4 * team + x) ^ (r0 & 7)) << 4)) = pack2<T>(e0, e1);
+                    *reinterpret_cast<uint32_t*>(pr + r1 * 128 + (((4 * team + x) ^ (r1 & 7)) << 4)) = pack2<T>(e2, e3);
+                    l0 += e0 + e1;
+                    l1 += e2 + e3;
                 }
                 if (p.seen - key0 < kTileKeys && p.seen % a.box_rows) {
                     // rows behind the sequence came with its last box: their weights are 0, and 0 times what lies there has to be 0
@@ -593,9 +633,9 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
                 }
                 proxy_fence();
                 tc_fence_before();
-                bar_arrive(&sh.p_full);
+                bar_arrive(&sh.p_full[s]);
             }
-            ok = ok && bar_wait(&sh.pv_done, (it - 1) & 1);
+            ok = ok && bar_wait(&sh.pv_done[(it - 1) & 1], (unsigned)((it - 1) >> 1) & 1);
             ok = !softmax_any(!ok);
             if (!ok) break;
             tc_fence_after();
@@ -604,10 +644,17 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
                 l0 += __shfl_xor_sync(0xffffffffu, l0, x);
                 l1 += __shfl_xor_sync(0xffffffffu, l1, x);
             }
+            if (team == 1 && (lane & 3) == 0) {
+                sh.team[1][r0] = l0;
+                sh.team[1][r1] = l1;
+            }
+            softmax_sync();
             const bool whole = p.t0 == 0 && p.t1 == p.tiles;
             const int slot = 2 * blockIdx.x + (p.t0 == 0 ? 1 : 0);
-            if ((lane & 3) == 0) {
+            if (team == 0 && (lane & 3) == 0) {
                 const int row0 = p.rb * kTileRows + r0, row1 = row0 + 8;
+                l0 += sh.team[1][r0];
+                l1 += sh.team[1][r1];
                 if (whole) {
                     sh.inv[r0] = l0 == 0.f ? 0.f : 1.f / l0;
                     sh.inv[r1] = l1 == 0.f ? 0.f : 1.f / l1;
@@ -626,12 +673,12 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
                 const int last = (int)((behind * plan.shares + plan.total - 1) / plan.total) - 1;
                 a.owner[blockIdx.x] = make_int4(p.b, p.rb, last - plan.share + 1, 0);
             }
-            softmax_sync();
             const int d0 = 32 * w + lane;
             if (whole) {
+                softmax_sync();
                 const int n = min(kTileRows, rows_all - p.rb * kTileRows);
 #pragma unroll 1
-                for (int x = 0; x < 8; ++x) {
+                for (int x = 4 * team; x < 4 * team + 4; ++x) {
                     uint32_t o[32];
                     tmem_ld_32x32(tmem + 32 * x + quarter, o);
                     tmem_ld_wait();
@@ -647,7 +694,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
             } else {
                 float* out = a.part_o + slot * kPartFloats + d0;
 #pragma unroll 1
-                for (int x = 0; x < 8; ++x) {
+                for (int x = 4 * team; x < 4 * team + 4; ++x) {
                     uint32_t o[32];
                     tmem_ld_32x32(tmem + 32 * x + quarter, o);
                     tmem_ld_wait();
