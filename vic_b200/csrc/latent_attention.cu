@@ -9,14 +9,15 @@
 // What bounds it: a cache row of 1152 bytes serves 2 (576 + 512) flops per row r, 121 flops per byte with 64 heads, half of
 // what the card does per byte; so HBM, as long as the tensor pipe keeps up.  Warp-level MMAs (about a third of the tcgen05
 // rate) do not.  Hence per tile of 64 keys and block of 64 rows, one CTA per SM:
-//   S [64 rows x 64 keys]  = Q . C^T      tcgen05, M = 64, K = 576; Q stays in shared memory for the whole sequence
-//   P = exp(S - m)                        four warps, from tensor memory to shared memory as 16-bit values
+//   S [64 rows x 64 keys]  = Q . C^T      tcgen05, M = 64, K = 576; Q stays in the SM for the whole sequence
+//   P = exp(S - m)                        eight warps, from tensor memory to shared memory as 16-bit values
 //   O^T [512 x 64 rows]   += C^T . P^T    tcgen05, four products with M = 128 values and N = 64 rows
 // The tile of C that TMA brought once is operand of both products: K-major (its 576 values contiguous) in the first, and in the
 // second, through another descriptor of the same bytes, MN-major.  With the accumulator transposed its 256 columns fill all 128
-// lanes of tensor memory, so it stays there for the whole sequence, and the number of rows is the N of the MMA.  Q (72 KB), two
-// tiles (144 KB) and P (8 KB) are all of shared memory; the tiles are handed over in five pieces of 128 (64) values, so that a
-// piece is refilled as soon as its product has read it.
+// lanes of tensor memory, so it stays there for the whole sequence, and the number of rows is the N of the MMA.
+// Per tile the pipe is busy 36 x 32 + 16 x 48 = 1920 cycles, HBM's share of an SM 3150.  What decides is how long a tile stays in
+// shared memory: load 2800 to 3500, S 1150, softmax 700, O 900 cycles.  With all of Q in shared memory there is room for two tiles
+// and a tile took 3500 cycles; with six of its nine chunks in tensor memory for two and three quarters.
 #include <cuda.h>
 
 #include "latent_common.cuh"
@@ -29,16 +30,27 @@ constexpr int kTileKeys = 64, kTileRows = 64;
 constexpr int kChunkBytes = 64 * 128;                     // 64 rows of 64 values, 128-byte swizzle
 constexpr int kChunks = kLatentRow / 64;                  // 9: eight of the latent, one of position values
 constexpr int kTileBytes = kChunks * kChunkBytes;
-constexpr int kGroups = 5;                                // pieces of a tile: chunk pairs 0..3, the position chunk
-constexpr int kQOff = 0, kKvOff = kTileBytes, kPOff = 8 * kChunkBytes /* in a tile */, kMiscOff = 3 * kTileBytes;
-constexpr int kAttThreads = 384;                          // copies, MMAs, two warps for Q, eight for the softmax and the results
+// Shared memory: the part of Q that tensor memory has no room for, a ring of latent chunk pairs, places for position values (then P).
+constexpr int kQTmemChunks = 6, kSlots = 11, kTiles = 3, kSlotBytes = 2 * kChunkBytes;
+constexpr int kQOff = 0, kRingOff = (kChunks - kQTmemChunks) * kChunkBytes, kRopeOff = kRingOff + kSlots * kSlotBytes;
+constexpr int kMiscOff = kRopeOff + kTiles * kChunkBytes;
+constexpr int kAttThreads = 384;                          // copies, S, O, (none), eight warps for Q, the softmax and the results
 constexpr int kSoftmaxThreads = 256;
-constexpr int kTmemCols = 512, kSCol = 256;               // O^T: 4 x 64 columns, S: 2 x 64
+constexpr int kTmemCols = 512, kSCol = 256, kQCol = 320;  // O^T: 4 x 64 columns, S: 64, Q: 6 x 32
+static_assert(kQCol + 32 * kQTmemChunks <= kTmemCols, "tensor memory");
 // The reference m of a row follows its maximum only when that has grown by more than 2^8: exp(s - m) then stays below 256, the
 // 16-bit weights keep their relative precision, and the accumulator is rescaled a few times per sequence instead of per tile.
 constexpr float kLazy = 8.0f;
 constexpr int kMaxGrid = 160;                             // CTAs that the workspace has room for
 constexpr size_t kPartFloats = (size_t)kTileRows * kRank;
+
+// Exact n / d for 0 <= n < 2^bits (bits <= 31) by one wide multiplication: mul = ceil(2^shift / d) with shift = bits + ceil(log2 d)
+// is off by less than d / 2^shift of a unit, so n * (the error) stays below 2^-s.  (A division instruction sequence is some twenty instructions,
+// and this kernel's code is fetched cold at every launch.)
+struct FastDiv {
+    unsigned mul, shift;
+    __device__ __forceinline__ int operator()(int n) const { return (int)((unsigned long long)(unsigned)n * mul >> shift); }
+};
 
 struct AttentionArgs {
     const void* q;
@@ -49,6 +61,7 @@ struct AttentionArgs {
     int table_stride, max_pages;
     const int* seq_lens;
     int batch, q_len, heads;
+    FastDiv by_heads, by_page;             // of rows (< 2^27), of keys (< 2^31)
     float scale_log2;                      // scale * log2(e)
     void* out;
     long long out_token, out_head;
@@ -59,7 +72,7 @@ struct AttentionArgs {
     // workspace: what CTA c owes to a sequence that other CTAs share, two slots per CTA
     int4* owner;                           // [grid] sequence, row block, parts (0: none)
     float2* part_ml;                       // [2 grid][64] reference (log2) and sum
-    float* part_o;                         // [2 grid][64][512], not yet divided by the sum
+    float4* part_o;                        // [2 grid][4][8][8][32] x 4 rows: 64 x 512 values, not yet divided by the sum
 };
 
 // The split.  A sequence has row blocks of 64 rows, a row block as many tiles as its last row sees.  Few row blocks (lanes =
@@ -67,64 +80,62 @@ struct AttentionArgs {
 // comes from HBM once.  Many: one lane, and a sequence's row blocks follow one another.  Within a lane the tiles of all sequences form one line that
 // is cut into equal shares whatever the lengths are; a sequence that a cut divides leaves parts that a second launch adds up.
 struct Plan {
-    long long begin, end, total;           // this CTA's tiles on the line
-    long long prefix;                      // of the first item
-    int item, lane, share, shares;
+    int begin, end;                        // this CTA's tiles on the line
+    int prefix, b, rb;                     // the first item: where it begins, sequence, row block
+    int share, shares, per, rem;           // share s begins at s * per + min(s, rem)
 };
 
 struct Piece {
     int b, rb, seen, tiles;                // item: sequence, row block, keys of its last row, tiles
     int t0, t1;                            // this CTA's tiles of it
-    long long prefix;
+    int prefix;
 };
 
-__device__ __forceinline__ int item_count(const AttentionArgs& a) { return a.batch * a.blocks_per_lane; }
+__device__ __forceinline__ int first_tile(const Plan& p, int share) { return share * p.per + min(share, p.rem); }
 
-__device__ __forceinline__ void item_of(const AttentionArgs& a, int lane, int item, Piece& p) {
-    p.b = a.blocks_per_lane == 1 ? item : item / a.blocks_per_lane;
-    p.rb = lane * a.blocks_per_lane + (item - p.b * a.blocks_per_lane);
-    const int last_row = min(a.q_len * a.heads, (p.rb + 1) * kTileRows) - 1;
-    const int len = max(__ldg(a.seq_lens + p.b), 0);
-    p.seen = min(max(len - a.q_len + last_row / a.heads + 1, 0), a.max_pages * a.page_size);
+__device__ __forceinline__ void item_of(const AttentionArgs& a, int b, int rb, Piece& p) {
+    p.b = b;
+    p.rb = rb;
+    const int last_row = min(a.q_len * a.heads, (rb + 1) * kTileRows) - 1;
+    const int len = max(__ldg(a.seq_lens + b), 0);
+    p.seen = min(max(len - a.q_len + a.by_heads(last_row) + 1, 0), a.max_pages * a.page_size);
     p.tiles = (p.seen + kTileKeys - 1) / kTileKeys;
 }
 
 // The pieces of this CTA in order.  Items without tiles belong to the CTA whose share they stand in (t0 == t1).
 struct Walk {
     const AttentionArgs& a;
-    const Plan& plan;
-    int item, items;
-    long long prefix;
-    __device__ __forceinline__ Walk(const AttentionArgs& a_, const Plan& p_) : a(a_), plan(p_), item(p_.item), items(item_count(a_)), prefix(p_.prefix) {}
-    __device__ __forceinline__ bool next(Piece& p, bool with_empty) {
-        const bool last = plan.share == plan.shares - 1;
-        while (item < items && (prefix < plan.end || last)) {
-            item_of(a, plan.lane, item, p);
-            p.prefix = prefix;
-            ++item;
-            prefix += p.tiles;
-            if (p.tiles == 0) {
-                p.t0 = p.t1 = 0;
-                if (with_empty) return true;
-                continue;
+    int b, rb, rb0, prefix, begin, end;
+    bool last;
+    __device__ __forceinline__ Walk(const AttentionArgs& a_, const Plan& p, int rb_first)
+        : a(a_), b(p.b), rb(p.rb), rb0(rb_first), prefix(p.prefix), begin(p.begin), end(p.end), last(p.share == p.shares - 1) {}
+    __device__ __forceinline__ bool next(Piece& p, bool empty) {
+#pragma unroll 1
+        while (b < a.batch && (prefix < end || last)) {
+            item_of(a, b, rb, p);
+            if (++rb == rb0 + a.blocks_per_lane) {
+                rb = rb0;
+                ++b;
             }
-            p.t0 = (int)max(plan.begin - p.prefix, 0ll);
-            p.t1 = (int)min(plan.end - p.prefix, (long long)p.tiles);
-            if (p.t1 > p.t0) return true;
+            p.prefix = prefix;
+            prefix += p.tiles;
+            p.t0 = max(begin - p.prefix, 0);
+            p.t1 = min(end - p.prefix, p.tiles);
+            if (p.tiles == 0 ? empty : !empty && p.t1 > p.t0) return true;
         }
         return false;
     }
 };
 
 struct AttShared {
-    uint64_t kv_full[2], kv_empty[2][kGroups];
-    uint64_t s_full[2], p_full[2], pv_done[2], q_full, q_empty, drain;
-    unsigned long long mask[2];            // keys of the tile that count
+    uint64_t kv_full[kTiles], slot_empty[kSlots], rope_empty[kTiles];
+    uint64_t s_full, s_free, p_full[2], pv_done[2], q_full, drain[2];
+    unsigned long long mask[kTiles];       // keys of the tile that count
     alignas(16) float factor[kTileRows];
     float team[2][kTileRows];              // what the two softmax teams have of a row: maximum, sum
     alignas(16) float inv[kTileRows];
     Plan plan;
-    long long warp_sum[kAttThreads / 32];
+    int warp_sum[kAttThreads / 32];
     uint32_t tmem;
 };
 static_assert(kMiscOff + sizeof(AttShared) <= 227 * 1024, "shared memory of a CTA");
@@ -149,19 +160,10 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, unsigned parity) {
                      : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
     return ok != 0;
 }
-// One look, without waiting; the warp's lanes agree.
-__device__ __forceinline__ bool bar_test(uint64_t* bar, unsigned parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    return __all_sync(0xffffffffu, ok != 0);
-}
-constexpr unsigned kIdleLimit = 1u << 26;   // looks without progress (each some 50 cycles: about two seconds)
 // The same for a whole warp, whose lanes have to agree (they meet again in warp-wide instructions).
 __device__ __forceinline__ bool bar_wait_warp(uint64_t* bar, unsigned parity) { return __all_sync(0xffffffffu, bar_wait(bar, parity)); }
-// 16 bytes global -> shared, zeros where !live
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 // One lane of the warp, the same one every time: behind elect.sync MMAs and tensor copies issue back to back.
 __device__ __forceinline__ bool elect_one() {
@@ -190,6 +192,12 @@ __device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
                  ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kDescHigh) : "memory");
 }
+// The same with the first operand in tensor memory.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kDescHigh) : "memory");
+}
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -199,6 +207,33 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// A row's log of its sum, from the reference (log2) and the sum relative to it; a part's weight relative to the largest reference.
+__device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994530942f; }
+__device__ __forceinline__ float weight_of(float part, float m) { return part == -INFINITY ? 0.f : ex2(part - m); }
+// 32 registers of a lane as eight groups of four: afterwards lane 4 q + s has of every group i the values that the lanes 4 q .. 4 q + 3
+// had in its register s.
+__device__ __forceinline__ void transpose4(uint32_t* o, int sub) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {      // lanes that differ in bit 0 exchange the off-diagonal registers of (e, e + 1)
+            const uint32_t give = sub & 1 ? o[i + e] : o[i + e + 1], got = __shfl_xor_sync(0xffffffffu, give, 1);
+            if (sub & 1) o[i + e] = got;
+            else o[i + e + 1] = got;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {         // bit 1: registers (e, e + 2)
+            const uint32_t give = sub & 2 ? o[i + e] : o[i + e + 2], got = __shfl_xor_sync(0xffffffffu, give, 2);
+            if (sub & 2) o[i + e] = got;
+            else o[i + e + 2] = got;
+        }
+    }
 }
 // Named barrier of the softmax warps; the second form tells whether any of them says so.
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory"); }
@@ -231,78 +266,81 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t* r)
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
 
-// This CTA's place on its lane's line of tiles.  All threads.  Up to kAttThreads items are read once and stay in registers.
+// This CTA's place on its lane's line of tiles.  All threads.  (The line has fewer than 2^31 tiles: checked by the launcher.)
 __device__ __forceinline__ void make_plan(const AttentionArgs& a, AttShared& sh) {
-    constexpr int kWarps = kAttThreads / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int row_lane = a.lanes == 1 ? 0 : blockIdx.x % a.lanes, share = a.lanes == 1 ? blockIdx.x : blockIdx.x / a.lanes, items = item_count(a);
-    const int most = a.lanes == 1 ? gridDim.x : gridDim.x / a.lanes;
+    const int row_lane = a.lanes == 1 ? 0 : blockIdx.x % a.lanes, share = a.lanes == 1 ? blockIdx.x : blockIdx.x / a.lanes;
+    const int most = a.lanes == 1 ? gridDim.x : gridDim.x / a.lanes, items = a.batch * a.blocks_per_lane;
     Piece p;
-    auto tiles_of = [&](int i) {
-        if (i >= items) return 0;
-        item_of(a, row_lane, i, p);
-        return p.tiles;
+    p.tiles = p.b = p.rb = 0;
+    auto look = [&](int i) {
+        const int b = a.blocks_per_lane == 1 ? i : i / a.blocks_per_lane;
+        item_of(a, b, row_lane * a.blocks_per_lane + i - b * a.blocks_per_lane, p);
     };
-    // inclusive sum over the block's threads; `sum` receives the total
-    auto block_scan = [&](long long v, long long& sum) {
+    // Pass 0 sums the tiles of all items, pass 1 finds the first item that begins at `begin` or reaches beyond it; a single chunk of
+    // items (the usual batch) needs no second look at the lengths.
+    int total = 0, begin = 0, end = 0, base = 0, pass = 0;
+#pragma unroll 1
+    for (int i0 = 0;;) {
+        const int i = i0 + tid;
+        if (i < items) look(i);
+        else p.tiles = 0;
+        int incl = p.tiles;
 #pragma unroll
         for (int m = 1; m < 32; m <<= 1) {
-            const long long o = __shfl_up_sync(0xffffffffu, v, m);
-            if (lane >= m) v += o;
+            const int o = __shfl_up_sync(0xffffffffu, incl, m);
+            if (lane >= m) incl += o;
         }
         __syncthreads();
-        if (lane == 31) sh.warp_sum[warp] = v;
+        if (lane == 31) sh.warp_sum[warp] = incl;
         __syncthreads();
-        sum = 0;
-        long long before = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w == warp) before = sum;
-            sum += sh.warp_sum[w];
+        int before = 0, chunk = 0;
+#pragma unroll 1
+        for (int w = 0; w < kAttThreads / 32; ++w) {
+            if (w == warp) before = chunk;
+            chunk += sh.warp_sum[w];
         }
-        return before + v;
-    };
-    const int first_tiles = tiles_of(tid);
-    long long mine = first_tiles, chunk, total;
-    for (int i = tid + kAttThreads; i < items; i += kAttThreads) mine += tiles_of(i);
-    long long incl = block_scan(mine, total);
-    const int shares = (int)max(1ll, min((long long)most, (total + a.min_tiles - 1) / a.min_tiles));
-    const bool idle = share >= shares;
-    // (a 64-bit division is a subroutine of some hundred instructions)
-    auto cut = [&](int k) {
-        return total <= 0x7fffffff / kMaxGrid ? (long long)((unsigned)total * (unsigned)k / (unsigned)shares) : total * k / shares;
-    };
-    const long long begin = idle ? total : cut(share), end = idle ? total : cut(share + 1);
-    if (tid == 0) {
-        sh.plan.begin = begin; sh.plan.end = end; sh.plan.total = total;
-        sh.plan.lane = row_lane; sh.plan.share = share; sh.plan.shares = shares;
-        if (idle) {
-            sh.plan.item = items;
-            sh.plan.prefix = total;
+        if (pass == 0) {
+            total += chunk;
+            if (i0 + kAttThreads < items) {
+                i0 += kAttThreads;
+                continue;
+            }
+            const int shares = max(1, min(most, (total + a.min_tiles - 1) / a.min_tiles));
+            const int per = total / shares, rem = total - per * shares;
+            begin = share * per + min(share, rem);
+            end = begin + per + (share < rem);
+            if (tid == 0) {
+                sh.plan.begin = begin; sh.plan.end = end; sh.plan.prefix = 0;
+                sh.plan.b = a.batch; sh.plan.rb = 0;      // (nothing, unless an item is found below)
+                sh.plan.share = share; sh.plan.shares = shares; sh.plan.per = per; sh.plan.rem = rem;
+            }
+            if (share >= shares) return;
+            pass = 1;
+            __syncthreads();
+            if (items > kAttThreads) {
+                i0 = 0;
+                continue;
+            }
         }
-    }
-    if (idle) return;
-    // the first item that begins at `begin` or reaches beyond it
-    long long base = 0;
-    for (int i0 = 0; i0 < items; i0 += kAttThreads) {
-        const int i = i0 + tid, tiles = i0 == 0 ? first_tiles : tiles_of(i);
-        if (items > kAttThreads) incl = block_scan(tiles, chunk);
-        else chunk = total;
-        const long long pre = base + incl - tiles;
-        // of those that qualify the first one: nothing before it begins at `begin`, and what comes before does not reach beyond
-        if (i < items && pre <= begin && (pre == begin || pre + tiles > begin)) {
+        const int pre = base + before + incl - p.tiles;
+        // of those that qualify the first one: with the beginning in common only items without tiles come before it
+        if (i < items && pre <= begin && (pre == begin || pre + p.tiles > begin)) {
+            const int b = p.b, rb = p.rb;
             bool first = true;
-            if (pre == begin && i > 0) {   // an item before this one with the same beginning (no tiles) comes first
-                item_of(a, row_lane, i - 1, p);
+            if (pre == begin && i > 0) {
+                look(i - 1);
                 first = p.tiles > 0;
             }
             if (first) {
-                sh.plan.item = i;
+                sh.plan.b = b;
+                sh.plan.rb = rb;
                 sh.plan.prefix = pre;
             }
         }
         base += chunk;
-        if (base > begin) break;
+        i0 += kAttThreads;
+        if (base > begin || i0 >= items) break;
     }
 }
 
@@ -313,16 +351,19 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
     const uint32_t base = smem_u32(smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     if (tid == 0) {
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < kSlots; ++s) bar_init(&sh.slot_empty[s], 1);
+        for (int s = 0; s < kTiles; ++s) {
             bar_init(&sh.kv_full[s], 1);
-            for (int g = 0; g < kGroups; ++g) bar_init(&sh.kv_empty[s][g], 1);
-            bar_init(&sh.s_full[s], 1);
+            bar_init(&sh.rope_empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
             bar_init(&sh.p_full[s], kSoftmaxThreads);
             bar_init(&sh.pv_done[s], 1);
+            bar_init(&sh.drain[s], 1);
         }
-        bar_init(&sh.q_full, 64);
-        bar_init(&sh.q_empty, 1);
-        bar_init(&sh.drain, 1);
+        bar_init(&sh.s_full, 1);
+        bar_init(&sh.s_free, kSoftmaxThreads);
+        bar_init(&sh.q_full, kSoftmaxThreads);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -338,25 +379,36 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
     const uint32_t tmem = uniform(sh.tmem);
     const Plan& plan = sh.plan;
     const int rows_all = a.q_len * a.heads;
-    Walk walk(a, plan);
+    Walk walk(a, plan, a.lanes == 1 ? 0 : (int)(blockIdx.x % a.lanes) * a.blocks_per_lane);
     Piece p;
     bool ok = (base & 1023) == 0;   // the swizzle is a function of the address
+    // tile `it` of this CTA: its latent chunk pairs lie in ring slots 4 it .. 4 it + 3 (mod kSlots), its position values in place it mod kTiles
+    int it = 0, slot = 0, place = 0;
+    unsigned place_parity = 0;
+    auto advance = [&] {
+        ++it;
+        slot += 4;
+        if (slot >= kSlots) slot -= kSlots;
+        if (++place == kTiles) {
+            place = 0;
+            place_parity ^= 1;
+        }
+    };
+    auto slot_of = [&](int g) { return slot + g >= kSlots ? slot + g - kSlots : slot + g; };
 
     if (warp == 0) {
         // ── copies: the tiles of C, in boxes of box_rows rows that lie in one page ──
         const int R = a.box_rows, nb = kTileKeys / R, per_load = 32 / nb;
-        int it = 0;
+        unsigned wraps = 0;                        // of the slots
         while (ok && walk.next(p, false)) {
             int page_of = 0, loaded = -1;
-            for (int t = p.t0; ok && t < p.t1; ++t, ++it) {
+            for (int t = p.t0; ok && t < p.t1; ++t) {
                 if (loaded < 0 || t >= loaded + per_load) {   // table entries of the next 32 boxes
                     loaded = t;
                     const int key = t * kTileKeys + lane * R;
-                    page_of = key < p.seen ? __ldg(a.page_table + (long long)p.b * a.table_stride + key / a.page_size) : -1;
+                    page_of = key < p.seen ? __ldg(a.page_table + (long long)p.b * a.table_stride + a.by_page(key)) : -1;
                 }
-                const int s = it & 1, key0 = t * kTileKeys;
-                const unsigned use = (unsigned)it >> 1;
-                const int src = min((t - loaded) * nb + lane, 31);
+                const int key0 = t * kTileKeys, src = min((t - loaded) * nb + lane, 31);
                 const int page = __shfl_sync(0xffffffffu, page_of, src), key = key0 + lane * R;
                 const bool mine = lane < nb, live = mine && key < p.seen, good = live && page >= 0 && page < a.num_pages;
                 if (live && !good && a.status) atomicOr(a.status, kStatusBadPage);
@@ -364,179 +416,274 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
                 unsigned long long m = (unsigned long long)__reduce_or_sync(0xffffffffu, (unsigned)(bits >> 32)) << 32 |
                                        __reduce_or_sync(0xffffffffu, (unsigned)bits);
                 if (p.seen - key0 < 64) m &= (1ull << (p.seen - key0)) - 1;
-                const int y = key % a.page_size, z = good ? page : a.num_pages;   // z = num_pages: outside, read as zeros
-                const uint32_t dst = base + kKvOff + s * kTileBytes + lane * R * 128;
-#pragma unroll
-                for (int g = 0; g < kGroups; ++g) {
-                    if (use > 0 && !bar_wait_warp(&sh.kv_empty[s][g], (use - 1) & 1)) {
-                        // the tile's remaining bytes will not come: what was requested is waited for below, this tile cannot be
+                const int y = key - a.by_page(key) * a.page_size, z = good ? page : a.num_pages;   // z = num_pages: outside, read as zeros
+                const uint32_t row = lane * R * 128;
+#pragma unroll 1
+                for (int g = 0; g < 5; ++g) {
+                    const int sl = slot_of(g);
+                    const unsigned w = wraps + (slot + g >= kSlots);
+                    uint64_t* const bar = g < 4 ? &sh.slot_empty[sl] : &sh.rope_empty[place];
+                    if ((g < 4 ? w > 0 : it >= kTiles) && !bar_wait_warp(bar, g < 4 ? (w - 1) & 1 : place_parity ^ 1)) {
                         ok = false;
                         break;
                     }
                     if (g == 0) {
                         if (lane == 0) {
-                            sh.mask[s] = m;
-                            bar_expect(&sh.kv_full[s], kTileBytes);
+                            sh.mask[place] = m;
+                            bar_expect(&sh.kv_full[place], kTileBytes);
                         }
                         __syncwarp();
                     }
                     if (mine) {
-                        tma_load_3d(dst + 2 * g * kChunkBytes, &map, 2 * g * 64, y, z, &sh.kv_full[s]);
-                        if (g < 4) tma_load_3d(dst + (2 * g + 1) * kChunkBytes, &map, (2 * g + 1) * 64, y, z, &sh.kv_full[s]);
+                        const uint32_t dst = base + row + (g < 4 ? kRingOff + sl * kSlotBytes : kRopeOff + place * kChunkBytes);
+                        tma_load_3d(dst, &map, 2 * g * 64, y, z, &sh.kv_full[place]);
+                        if (g < 4) tma_load_3d(dst + kChunkBytes, &map, (2 * g + 1) * 64, y, z, &sh.kv_full[place]);
                     }
                     __syncwarp();
                 }
+                if (slot + 4 >= kSlots) ++wraps;
+                advance();
             }
         }
         // Nothing is owed to this CTA's memory when it leaves: the releases of the last tiles arrive, or, after a wait that ran out,
         // the copies in flight do (the newest tile's barrier may lack bytes that were never requested: that wait gives up).
-        for (int n = max(it - 2, 0); n < it; ++n)
-            for (int g = 0; g < kGroups; ++g)
-                if (!ok || !bar_wait_warp(&sh.kv_empty[n & 1][g], (n >> 1) & 1)) {
-                    ok = false;
-                    bar_wait_warp(&sh.kv_full[n & 1], (n >> 1) & 1);
-                    break;
-                }
+#pragma unroll 1
+        for (int s = 0; ok && s < kSlots; ++s) {
+            const int uses = 4 * it / kSlots + (s < 4 * it % kSlots);
+            if (uses > 0) ok = bar_wait_warp(&sh.slot_empty[s], (uses - 1) & 1);
+        }
+#pragma unroll 1
+        for (int s = 0; s < kTiles; ++s) {
+            const int uses = it / kTiles + (s < it % kTiles);
+            if (uses > 0 && ok) ok = bar_wait_warp(&sh.rope_empty[s], (uses - 1) & 1);
+            if (uses > 0 && !ok) bar_wait_warp(&sh.kv_full[s], (uses - 1) & 1);
+        }
     } else if (warp == 1) {
-        // ── MMAs ──
-        // Two walks over the same tiles, S at most two tiles ahead of O (its two buffers).  Whatever has its operands goes next, O
-        // first, since only O gives shared memory back: with S(i + 1) always before O(i), O waited for the load of tile i + 1,
-        // which waits for the room of tile i - 1, and a tile took 4100 cycles.
-        Walk walk_o(a, plan);
-        Piece po;
-        bool more_s = ok && walk.next(p, false), more_o = ok && walk_o.next(po, false);
-        int ns = 0, ts = p.t0, q_pieces = 0;              // next S: tile count, tile of the item, pieces whose Q was read
-        int no = 0, to = po.t0;                           // next O
-        bool q_ready = false;
-        unsigned idle = 0;
-        while (more_o) {
-            if (no < ns && bar_test(&sh.p_full[no & 1], (no >> 1) & 1)) {
+        // ── S = Q . C^T ──
+        int pieces = 0;
+        while (ok && walk.next(p, false)) {
+            ok = bar_wait_warp(&sh.q_full, pieces & 1);
+            for (int t = p.t0; ok && t < p.t1; ++t) {
+                ok = bar_wait_warp(&sh.kv_full[place], place_parity) && (it == 0 || bar_wait_warp(&sh.s_free, (it - 1) & 1));
+                if (!ok) break;
                 tc_fence_after();
-                const int st = (int)uniform((uint32_t)no & 1);
-                const uint32_t c = uniform(base + kKvOff + st * kTileBytes), v = desc_mn(c), pk = desc_k(c + kPOff), acc = uniform(to > po.t0);
+                const uint32_t d = tmem + kSCol, qt = tmem + kQCol, qd = uniform(desc_k(base + kQOff));
+                uint32_t cd[5];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) cd[g] = uniform(desc_k(base + kRingOff + slot_of(g) * kSlotBytes));
+                cd[4] = uniform(desc_k(base + kRopeOff + place * kChunkBytes));
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < 4 * kChunks; ++k) {
+                        const int c = k >> 2;
+                        const uint32_t b = cd[c >> 1] + (c & 1) * (kChunkBytes / 16) + (k & 3) * 2;
+                        if (c < kQTmemChunks) umma_ts(d, qt + 8 * k, b, kIdescS<T>, k > 0);
+                        else umma_ss(d, qd + (c - kQTmemChunks) * (kChunkBytes / 16) + (k & 3) * 2, b, kIdescS<T>, 1u);
+                    }
+                    umma_commit(&sh.s_full);
+                }
+                __syncwarp();
+                advance();
+            }
+            ++pieces;
+        }
+        if (!ok) {   // the MMAs that were issued have to be through before the tensor memory is freed
+            if (elect_one()) umma_commit(&sh.drain[0]);
+            __syncwarp();
+            bar_wait_warp(&sh.drain[0], 0);
+        }
+    } else if (warp == 2) {
+        // ── O^T += C^T . P^T ──
+        while (ok && walk.next(p, false)) {
+            for (int t = p.t0; ok && t < p.t1; ++t) {
+                ok = bar_wait_warp(&sh.kv_full[place], place_parity) && bar_wait_warp(&sh.p_full[it & 1], (unsigned)(it >> 1) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t pd = uniform(desc_k(base + kRopeOff + place * kChunkBytes)), acc = uniform(t > p.t0);
+                uint32_t cd[4];
+                int sl[4];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    sl[g] = (int)uniform((uint32_t)slot_of(g));
+                    cd[g] = uniform(desc_mn(base + kRingOff + sl[g] * kSlotBytes));
+                }
                 if (elect_one()) {
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            umma_ss(tmem + 64 * g, v + (2 * g * kChunkBytes + k * 2048) / 16, pk + k * 2, kIdescO<T>, k > 0 ? 1u : acc);
-                        umma_commit(&sh.kv_empty[st][g]);
+                        for (int k = 0; k < 4; ++k) umma_ss(tmem + 64 * g, cd[g] + k * (2048 / 16), pd + k * 2, kIdescO<T>, k > 0 ? 1u : acc);
+                        umma_commit(&sh.slot_empty[sl[g]]);
                     }
-                    umma_commit(&sh.kv_empty[st][kGroups - 1]);
-                    umma_commit(&sh.pv_done[st]);
+                    umma_commit(&sh.rope_empty[place]);
+                    umma_commit(&sh.pv_done[it & 1]);
                 }
                 __syncwarp();
-                ++no;
-                if (++to == po.t1) {
-                    more_o = walk_o.next(po, false);
-                    to = po.t0;
-                }
-                idle = 0;
-                continue;
-            }
-            if (more_s && ns < no + 2) {
-                if (!q_ready && bar_test(&sh.q_full, q_pieces & 1)) q_ready = true;
-                if (q_ready && bar_test(&sh.kv_full[ns & 1], (ns >> 1) & 1)) {
-                    tc_fence_after();
-                    const bool piece_end = ts + 1 == p.t1;
-                    const int st = (int)uniform((uint32_t)ns & 1);
-                    const uint32_t d = uniform(tmem + kSCol + 64 * st), qd = uniform(desc_k(base + kQOff)), cd = uniform(desc_k(base + kKvOff + st * kTileBytes));
-                    if (elect_one()) {
-#pragma unroll
-                        for (int k = 0; k < 4 * kChunks; ++k)
-                            umma_ss(d, qd + (k >> 2) * kChunkBytes / 16 + (k & 3) * 2, cd + (k >> 2) * kChunkBytes / 16 + (k & 3) * 2, kIdescS<T>, k > 0);
-                        umma_commit(&sh.s_full[st]);
-                        if (piece_end) umma_commit(&sh.q_empty);
-                    }
-                    __syncwarp();
-                    ++ns;
-                    ++ts;
-                    if (piece_end) {
-                        q_ready = false;
-                        ++q_pieces;
-                        more_s = walk.next(p, false);
-                        ts = p.t0;
-                    }
-                    idle = 0;
-                    continue;
-                }
-            }
-            if (++idle > kIdleLimit) {
-                ok = false;
-                break;
+                advance();
             }
         }
-        if (!ok) {   // the MMAs that were issued have to be through before the tensor memory is freed
-            if (elect_one()) umma_commit(&sh.drain);
+        if (!ok) {
+            if (elect_one()) umma_commit(&sh.drain[1]);
             __syncwarp();
-            bar_wait_warp(&sh.drain, 0);
+            bar_wait_warp(&sh.drain[1], 0);
         }
-    } else if (warp < 4) {
-        // ── Q of a piece: 64 rows, zeros behind the last one ──
-        int pieces = 0;
-        while (ok && walk.next(p, false)) {
-            if (pieces > 0) ok = bar_wait_warp(&sh.q_empty, (pieces - 1) & 1);
-            if (!ok) break;
-            const long long token0 = (long long)p.b * a.q_len;
-            // A warp takes every second row; lane i works out the address of its i-th (a division per 16 bytes: 8 us per piece).
-            const int row = p.rb * kTileRows + 2 * lane + (warp & 1), j = row / a.heads, h = row - j * a.heads;
-            const long long at = row < rows_all ? (token0 + j) * a.q_token + h * a.q_head : -1;
-            const uint32_t piece = (uint32_t)(lane & 7), chunk = base + kQOff + (lane >> 3) * kChunkBytes;
-#pragma unroll 8
-            for (int i = 0; i < kTileRows / 2; ++i) {
-                const long long off = __shfl_sync(0xffffffffu, at, i);
-                const bool live = off >= 0;
-                const T* src = (const T*)a.q + (live ? off : 0) + lane * 8;
-                const int r = 2 * i + (warp & 1);
-                const uint32_t dst = chunk + r * 128 + ((piece ^ (r & 7)) << 4);
-                cp_async16(dst, src, live);
-                cp_async16(dst + 4 * kChunkBytes, src + 256, live);
-                if (lane < 8) cp_async16(dst + 8 * kChunkBytes, src + 512, live);
+    } else if (warp == 3) {
+        // ── Q of the later pieces into L2: fetched from HBM under the streaming tiles it took 5000 cycles between two pieces ──
+        for (bool first = true; ok && walk.next(p, false); first = false) {
+            if (first) continue;
+            for (int r = lane; r < kTileRows; r += 32) {
+                const int row = p.rb * kTileRows + r, j = a.by_heads(row);
+                if (row >= rows_all) break;
+                const T* q = (const T*)a.q + ((long long)p.b * a.q_len + j) * a.q_token + (row - j * a.heads) * a.q_head;
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + 64 * c));
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            proxy_fence();
-            bar_arrive(&sh.q_full);
-            ++pieces;
         }
-        if (ok && pieces > 0) ok = bar_wait(&sh.q_empty, (pieces - 1) & 1);
     } else {
-        // ── softmax and results ──
+        // ── Q, softmax and results ──
         // Two teams of four warps, 32 keys each; warp w of a team has rows 16 w .. (their lanes in tensor memory), a thread two rows
         // and eight keys of each.  (A thread whose wait ran out goes on to the next common barrier, where all of them leave.)
         const int team = (warp - 4) >> 2, w = warp & 3, r0 = 16 * w + (lane >> 2), r1 = r0 + 8, c0 = 32 * team + 2 * (lane & 3);
         const uint32_t quarter = (uint32_t)(32 * w) << 16;
         const int stid = tid - 128;
-        if (stid == 0) a.owner[blockIdx.x] = make_int4(0, 0, 0, 0);
-        int it = 0;
-        while (ok && walk.next(p, true)) {
-            const int len = max(__ldg(a.seq_lens + p.b), 0);
-            const long long token0 = (long long)p.b * a.q_len;
-            if (stid == 0 && len > a.max_pages * a.page_size && a.status) atomicOr(a.status, kStatusBadPage);
-            if (p.tiles == 0) {      // no row of the block sees a key
-                const int n = min(kTileRows, rows_all - p.rb * kTileRows);
-                for (int r = warp - 4; r < n; r += 8) {
-                    const int row = p.rb * kTileRows + r, j = row / a.heads, h = row - j * a.heads;
-                    uint4* o = reinterpret_cast<uint4*>((T*)a.out + (token0 + j) * a.out_token + h * a.out_head);
-                    o[lane] = o[lane + 32] = make_uint4(0, 0, 0, 0);
-                    if (lane == 0 && a.lse) a.lse[(token0 + j) * a.heads + h] = -INFINITY;
-                }
-                continue;
+        // Q of a piece (behind its last row that row again: what comes of it is not stored): six chunks of its nine to tensor memory (row 16 w + i is lane 32 w + i, two
+        // values per column), three to shared memory.  Its place is free: the scores of the piece before have been seen.
+        auto load_q = [&](const Piece& n) {
+            const T* q = (const T*)a.q + (long long)n.b * a.q_len * a.q_token;
+            auto row_at = [&](int r) {
+                const int row = min(n.rb * kTileRows + r, rows_all - 1), j = a.by_heads(row);
+                return q + j * a.q_token + (row - j * a.heads) * a.q_head;
+            };
+            const T* src = row_at(16 * w + (lane & 15)) + 3 * team * 64;
+            uint4 v[3][8];
+#pragma unroll
+            for (int c = 0; c < 3; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[c][i] = __ldg(reinterpret_cast<const uint4*>(src + c * 64 + i * 8));
+            if (lane < 24) {
+                const uint32_t dst = base + kQOff + (lane >> 3) * kChunkBytes + 8 * (warp - 4) * 128;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) cp_async16(dst + i * 128 + (((lane & 7) ^ i) << 4), row_at(8 * (warp - 4) + i) + kQTmemChunks * 64 + lane * 8);
             }
-            const int j0 = (p.rb * kTileRows + r0) / a.heads, j1 = (p.rb * kTileRows + r1) / a.heads;
+#pragma unroll
+            for (int c = 0; c < 3; ++c) tmem_st_32x32(tmem + kQCol + 32 * (3 * team + c) + quarter, reinterpret_cast<const uint32_t*>(v[c]));
+            tmem_st_wait();
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            proxy_fence();
+            tc_fence_before();
+            bar_arrive(&sh.q_full);
+        };
+        if (stid == 0) a.owner[blockIdx.x] = make_int4(0, 0, 0, 0);
+        // A round: the next piece's Q (under the last product of the piece before), that piece's results, the next one's tiles.
+        float m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f;
+        long long token0 = 0;
+        Piece next;
+#pragma unroll 1
+        for (bool open = false; open || ok; open = true) {
+            const bool more = walk.next(next, false);
+            if (more) load_q(next);
+            if (open) {
+                ok = ok && bar_wait(&sh.pv_done[(it - 1) & 1], (unsigned)((it - 1) >> 1) & 1);
+                ok = !softmax_any(!ok);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int x = 1; x < 4; x <<= 1) {
+                    l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+                    l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+                }
+                if (team == 1 && (lane & 3) == 0) {
+                    sh.team[1][r0] = l0;
+                    sh.team[1][r1] = l1;
+                }
+                softmax_sync();
+                const bool whole = p.t0 == 0 && p.t1 == p.tiles;
+                const int part = 2 * blockIdx.x + (p.t0 == 0 ? 1 : 0);
+                if (team == 0 && (lane & 3) == 0) {
+                    const int row0 = p.rb * kTileRows + r0, row1 = row0 + 8;
+                    l0 += sh.team[1][r0];
+                    l1 += sh.team[1][r1];
+                    if (whole) {
+                        sh.inv[r0] = l0 == 0.f ? 0.f : rcp(l0);
+                        sh.inv[r1] = l1 == 0.f ? 0.f : rcp(l1);
+                        if (a.lse) {
+                            if (row0 < rows_all) a.lse[token0 * a.heads + row0] = lse_of(m0, l0);
+                            if (row1 < rows_all) a.lse[token0 * a.heads + row1] = lse_of(m1, l1);
+                        }
+                    } else {
+                        a.part_ml[part * kTileRows + r0] = make_float2(m0, l0);
+                        a.part_ml[part * kTileRows + r1] = make_float2(m1, l1);
+                    }
+                }
+                if (!whole && p.t0 == 0 && stid == 0) {
+                    // the share that holds the item's last tile
+                    const int x = p.prefix + p.tiles - 1, wide = plan.rem * (plan.per + 1);
+                    const int last = x < wide ? x / (plan.per + 1) : plan.rem + (x - wide) / plan.per;
+                    a.owner[blockIdx.x] = make_int4(p.b, p.rb, last - plan.share + 1, 0);
+                }
+                if (whole) {
+                    softmax_sync();
+                    const int n = min(kTileRows, rows_all - p.rb * kTileRows), sub = lane & 3;
+#pragma unroll 1
+                    for (int x = 4 * team; x < 4 * team + 4; ++x) {
+                        uint32_t o[32];
+                        tmem_ld_32x32(tmem + 32 * x + quarter, o);
+                        tmem_ld_wait();
+                        // a lane has one value of 32 rows; four lanes exchange theirs, so that each has four neighbouring values of eight rows
+                        transpose4(o, sub);
+                        int r = 32 * (x & 1) + sub;
+                        T* out = (T*)a.out + token0 * a.out_token + 128 * (x >> 1) + 32 * w + (lane & ~3);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i, r += 4) {
+                            if (r < n) {
+                                const int row = p.rb * kTileRows + r, j = a.by_heads(row), h = row - j * a.heads;
+                                const float f = sh.inv[r];
+                                uint2 b;
+                                b.x = pack2<T>(__uint_as_float(o[4 * i]) * f, __uint_as_float(o[4 * i + 1]) * f);
+                                b.y = pack2<T>(__uint_as_float(o[4 * i + 2]) * f, __uint_as_float(o[4 * i + 3]) * f);
+                                *reinterpret_cast<uint2*>(out + j * a.out_token + h * a.out_head) = b;
+                            }
+                        }
+                    }
+                } else {
+                    // in the order in which the values lie in registers: four rows of a value are 16 bytes, a warp's 32 values 512
+                    float4* out = a.part_o + (size_t)part * (kPartFloats / 4) + w * (8 * 8 * 32) + lane;
+#pragma unroll 1
+                    for (int x = 4 * team; x < 4 * team + 4; ++x) {
+                        uint32_t o[32];
+                        tmem_ld_32x32(tmem + 32 * x + quarter, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            out[(x * 8 + i) * 32] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                                                                __uint_as_float(o[4 * i + 3]));
+                    }
+                }
+                tc_fence_before();
+            }
+            if (!more) break;
+            p = next;
+            const int len = max(__ldg(a.seq_lens + p.b), 0);
+            token0 = (long long)p.b * a.q_len;
+            if (stid == 0 && len > a.max_pages * a.page_size && a.status) atomicOr(a.status, kStatusBadPage);
+            const int j0 = a.by_heads(p.rb * kTileRows + r0), j1 = a.by_heads(p.rb * kTileRows + r1);
             const int seen0 = min(len - a.q_len + j0 + 1, p.seen), seen1 = min(len - a.q_len + j1 + 1, p.seen);
-            const int seen_all = min(len - a.q_len + p.rb * kTileRows / a.heads + 1, p.seen);    // keys that every row sees
-            float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-            for (int t = p.t0; t < p.t1; ++t, ++it) {
-                const int s = it & 1, key0 = t * kTileKeys;
-                const unsigned parity = (unsigned)(it >> 1) & 1;
-                // (the tile two before is through when this one's scores are; seen here, its phase cannot be taken for another)
-                ok = ok && (it < 2 || bar_wait(&sh.pv_done[s], parity ^ 1)) && bar_wait(&sh.kv_full[s], parity) && bar_wait(&sh.s_full[s], parity);
+            const int seen_all = min(len - a.q_len + a.by_heads(p.rb * kTileRows) + 1, p.seen);    // keys that every row sees
+            m0 = m1 = -INFINITY;
+            l0 = l1 = 0.f;
+#pragma unroll 1
+            for (int t = p.t0; t < p.t1; ++t) {
+                const int key0 = t * kTileKeys;
+                // (waiting for O of the tile two before keeps its barrier's phases apart)
+                ok = ok && (it < 2 || bar_wait(&sh.pv_done[it & 1], (unsigned)((it >> 1) - 1) & 1)) && bar_wait(&sh.kv_full[place], place_parity) &&
+                     bar_wait(&sh.s_full, it & 1);
                 __syncwarp();
-                const unsigned long long mask = sh.mask[s];
+                const unsigned long long mask = sh.mask[place];
                 tc_fence_after();
                 uint32_t raw[16];
-                tmem_ld_16x32(tmem + kSCol + 64 * s + 32 * team + quarter, raw);
+                tmem_ld_16x32(tmem + kSCol + 32 * team + quarter, raw);
                 tmem_ld_wait();
+                tc_fence_before();
+                bar_arrive(&sh.s_free);
                 float v[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(raw[i]) * a.scale_log2;
@@ -585,13 +732,13 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
                         m1 = x1;
                         l1 *= f1;
                     }
-                    if (team == 0 && (lane & 3) == 0) {
-                        sh.factor[r0] = f0;
-                        sh.factor[r1] = f1;
-                    }
-                    softmax_sync();
                     if (t > p.t0) {
-                        ok = bar_wait(&sh.pv_done[s ^ 1], (unsigned)((it - 1) >> 1) & 1);
+                        if (team == 0 && (lane & 3) == 0) {
+                            sh.factor[r0] = f0;
+                            sh.factor[r1] = f1;
+                        }
+                        softmax_sync();
+                        ok = bar_wait(&sh.pv_done[(it - 1) & 1], (unsigned)((it - 1) >> 1) & 1);
                         __syncwarp();
                         tc_fence_after();
 #pragma unroll 1
@@ -615,7 +762,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
                 }
                 const float n0 = m0 == -INFINITY ? 0.f : m0, n1 = m1 == -INFINITY ? 0.f : m1;
                 // P takes the place of the tile's position values, which no product reads again
-                unsigned char* pr = smem + kKvOff + s * kTileBytes + kPOff + 4 * (lane & 3);
+                unsigned char* pr = smem + kRopeOff + place * kChunkBytes + 4 * (lane & 3);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     const float e0 = ex2(v[4 * x] - n0), e1 = ex2(v[4 * x + 1] - n0), e2 = ex2(v[4 * x + 2] - n1), e3 = ex2(v[4 * x + 3] - n1);
@@ -627,82 +774,30 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
                 if (p.seen - key0 < kTileKeys && p.seen % a.box_rows) {
                     // rows behind the sequence came with its last box: their weights are 0, and 0 times what lies there has to be 0
                     const int first = p.seen - key0, n = (kTileKeys - first) * 8;
+#pragma unroll 1
                     for (int c = 0; c < 8; ++c)
+#pragma unroll 1
                         for (int i = stid; i < n; i += kSoftmaxThreads)
-                            *reinterpret_cast<uint4*>(smem + kKvOff + s * kTileBytes + c * kChunkBytes + first * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(smem + kRingOff + slot_of(c >> 1) * kSlotBytes + (c & 1) * kChunkBytes + first * 128 + i * 16) =
+                                make_uint4(0, 0, 0, 0);
                 }
                 proxy_fence();
                 tc_fence_before();
-                bar_arrive(&sh.p_full[s]);
+                bar_arrive(&sh.p_full[it & 1]);
+                advance();
             }
-            ok = ok && bar_wait(&sh.pv_done[(it - 1) & 1], (unsigned)((it - 1) >> 1) & 1);
-            ok = !softmax_any(!ok);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int x = 1; x < 4; x <<= 1) {
-                l0 += __shfl_xor_sync(0xffffffffu, l0, x);
-                l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+        }
+        // Items of this CTA that have no tiles: no row of theirs sees a key.
+        Walk none(a, plan, walk.rb0);
+        while (ok && none.next(p, true)) {
+            const int n = min(kTileRows, rows_all - p.rb * kTileRows);
+            for (int r = warp - 4; r < n; r += 8) {
+                const int row = p.rb * kTileRows + r, j = a.by_heads(row), h = row - j * a.heads;
+                const long long token = (long long)p.b * a.q_len + j;
+                uint4* o = reinterpret_cast<uint4*>((T*)a.out + token * a.out_token + h * a.out_head);
+                o[lane] = o[lane + 32] = make_uint4(0, 0, 0, 0);
+                if (lane == 0 && a.lse) a.lse[token * a.heads + h] = -INFINITY;
             }
-            if (team == 1 && (lane & 3) == 0) {
-                sh.team[1][r0] = l0;
-                sh.team[1][r1] = l1;
-            }
-            softmax_sync();
-            const bool whole = p.t0 == 0 && p.t1 == p.tiles;
-            const int slot = 2 * blockIdx.x + (p.t0 == 0 ? 1 : 0);
-            if (team == 0 && (lane & 3) == 0) {
-                const int row0 = p.rb * kTileRows + r0, row1 = row0 + 8;
-                l0 += sh.team[1][r0];
-                l1 += sh.team[1][r1];
-                if (whole) {
-                    sh.inv[r0] = l0 == 0.f ? 0.f : 1.f / l0;
-                    sh.inv[r1] = l1 == 0.f ? 0.f : 1.f / l1;
-                    if (a.lse) {
-                        if (row0 < rows_all) a.lse[token0 * a.heads + row0] = l0 == 0.f ? -INFINITY : (m0 + log2f(l0)) * 0.69314718055994530942f;
-                        if (row1 < rows_all) a.lse[token0 * a.heads + row1] = l1 == 0.f ? -INFINITY : (m1 + log2f(l1)) * 0.69314718055994530942f;
-                    }
-                } else {
-                    a.part_ml[slot * kTileRows + r0] = make_float2(m0, l0);
-                    a.part_ml[slot * kTileRows + r1] = make_float2(m1, l1);
-                }
-            }
-            if (!whole && p.t0 == 0 && stid == 0) {
-                // the share that holds the item's last tile: the smallest s with total (s + 1) / shares beyond it
-                const long long behind = p.prefix + p.tiles;
-                const int last = (int)((behind * plan.shares + plan.total - 1) / plan.total) - 1;
-                a.owner[blockIdx.x] = make_int4(p.b, p.rb, last - plan.share + 1, 0);
-            }
-            const int d0 = 32 * w + lane;
-            if (whole) {
-                softmax_sync();
-                const int n = min(kTileRows, rows_all - p.rb * kTileRows);
-#pragma unroll 1
-                for (int x = 4 * team; x < 4 * team + 4; ++x) {
-                    uint32_t o[32];
-                    tmem_ld_32x32(tmem + 32 * x + quarter, o);
-                    tmem_ld_wait();
-                    const int rb = 32 * (x & 1);
-                    int j = (p.rb * kTileRows + rb) / a.heads, h = p.rb * kTileRows + rb - j * a.heads;
-                    T* out = (T*)a.out + 128 * (x >> 1) + d0;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        if (rb + i < n) out[(token0 + j) * a.out_token + h * a.out_head] = from_float<T>(__uint_as_float(o[i]) * sh.inv[rb + i]);
-                        if (++h == a.heads) { h = 0; ++j; }
-                    }
-                }
-            } else {
-                float* out = a.part_o + slot * kPartFloats + d0;
-#pragma unroll 1
-                for (int x = 4 * team; x < 4 * team + 4; ++x) {
-                    uint32_t o[32];
-                    tmem_ld_32x32(tmem + 32 * x + quarter, o);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) out[(32 * (x & 1) + i) * kRank + 128 * (x >> 1)] = __uint_as_float(o[i]);
-                }
-            }
-            tc_fence_before();
         }
     }
     if (!ok && lane == 0 && a.status) atomicOr(a.status, 4 /* VIB3_STATUS_TIMEOUT */);
@@ -714,62 +809,111 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
     }
 }
 
-// Adds up the parts of the sequences that several CTAs shared.  A block takes rows (owner, row) in turn: 128 threads cover the 512
-// values, four such teams take every fourth part.  Parts of an owner c lie in its second slot and in the first slots of the CTAs after it in its lane.
-constexpr int kCombineTeams = 4;
+// Adds up the parts of the sequences that several CTAs shared.  Parts of an owner c lie in its second place and in the first places of
+// the CTAs after it in its lane.  Every block lists the owners; a warp's work is four rows and 128 of the 512 values (of a part, each
+// value's four rows are 16 bytes).  With few parts it adds all of them; with many, a block's eight warps take every eighth part of the same
+// four rows and half of those values, and meet in shared memory.  It works out its rows' weights itself, so that nothing waits for
+// other warps.  (Both ways are needed: a warp for all parts took 100 us where one sequence had 148, a block per row 35 us where 128 sequences had two.)
+constexpr int kCombineFew = 8, kCombineThreads = 256;
 
 template <typename T>
-__global__ void __launch_bounds__(kCombineTeams * 128) latent_combine_kernel(const AttentionArgs a, int grid) {
-    __shared__ float weight[kMaxGrid];
-    __shared__ float4 sums[kCombineTeams - 1][128];
+__global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const AttentionArgs a, int grid) {
+    __shared__ int4 owners[kMaxGrid];
+    __shared__ int upto[kCombineThreads];      // blocks of work up to and with owner c
+    __shared__ int warp_sum[kCombineThreads / 32];
+    __shared__ float4 sums[kCombineThreads / 32][2][32];
     pdl_enter();
-    const int tid = threadIdx.x, team = tid >> 7, x = tid & 127;
-    for (int i = blockIdx.x; i < grid * kTileRows; i += gridDim.x) {
-        const int c = i / kTileRows, r = i % kTileRows;
-        const int4 own = a.owner[c];
-        const int row = own.y * kTileRows + r;
-        if (own.z == 0 || row >= a.q_len * a.heads) continue;
-        const int parts = own.z;
-        const long long token = (long long)own.x * a.q_len + row / a.heads;
-        const int h = row % a.heads;
-        if (tid < 32) {
-            float m = -INFINITY, l = 0.f;
-            for (int k = tid; k < parts; k += 32) m = fmaxf(m, a.part_ml[(2 * (c + k * a.lanes) + (k == 0)) * kTileRows + r].x);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rows_all = a.q_len * a.heads;
+    int units = 0;
+    if (tid < grid) {
+        const int4 own = a.owner[tid];
+        owners[tid] = own;
+        units = own.z == 0 ? 0 : own.z <= kCombineFew ? 8 : 128;
+    }
 #pragma unroll
-            for (int y = 16; y; y >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, y));
-            for (int k = tid; k < parts; k += 32) {
-                const float2 ml = a.part_ml[(2 * (c + k * a.lanes) + (k == 0)) * kTileRows + r];
-                const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
-                weight[k] = f;
-                l = fmaf(f, ml.y, l);
-            }
+    for (int m = 1; m < 32; m <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, units, m);
+        if (lane >= m) units += o;
+    }
+    if (lane == 31) warp_sum[warp] = units;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) units += warp_sum[w];
+    upto[tid] = units;
+    __syncthreads();
+    const int all = upto[kCombineThreads - 1];
+#pragma unroll 1
+    for (int u = blockIdx.x; u < all; u += gridDim.x) {
+        int c = 0;
 #pragma unroll
-            for (int y = 16; y; y >>= 1) l += __shfl_xor_sync(0xffffffffu, l, y);
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            __syncwarp();
-            for (int k = tid; k < parts; k += 32) weight[k] *= inv;
-            if (tid == 0 && a.lse) a.lse[token * a.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
-        }
-        __syncthreads();
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int step = kCombineThreads / 2; step; step >>= 1) c += upto[c + step - 1] <= u ? step : 0;
+        const int4 own = owners[c];
+        const int parts = own.z, x = u - (c ? upto[c - 1] : 0);
+        const bool few = parts <= kCombineFew;
+        // rows r .. r + 3 (of the block's 64), values 128 g + 32 w + lane with g in [g0, g0 + gn)
+        const int r = few ? (x * 2 + (warp >> 2)) * 4 : (x >> 3) * 4, w = few ? warp & 3 : (x >> 1) & 3, g0 = few ? 0 : 2 * (x & 1), gn = few ? 4 : 2;
+        const int row0 = own.y * kTileRows + r;
+        if (few && row0 >= rows_all) continue;     // (of the other kind all warps come to the barriers below)
+        auto place = [&](int k) { return 2 * (c + k * a.lanes) + (k == 0); };
+        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, l[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int k = lane; k < parts; k += 32)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], a.part_ml[place(k) * kTileRows + r + e].x);
+#pragma unroll
+        for (int y = 16; y; y >>= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], y));
+        float4 o[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) o[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4* src = a.part_o + (w * 64 + (2 * g0 + (r >> 5)) * 8 + ((r & 31) >> 2)) * 32 + lane;
 #pragma unroll 4
-        for (int k = team; k < parts; k += kCombineTeams) {
-            const float f = weight[k];
-            const float4 v = *reinterpret_cast<const float4*>(a.part_o + (2 * (c + k * a.lanes) + (k == 0)) * kPartFloats + r * kRank + 4 * x);
-            o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
-        }
-        if (team) sums[team - 1][x] = o;
-        __syncthreads();
-        if (team == 0) {
+        for (int k = few ? 0 : warp; k < parts; k += few ? 1 : kCombineThreads / 32) {
+            const float4* ml = reinterpret_cast<const float4*>(a.part_ml + place(k) * kTileRows + r);
+            const float4 p0 = ml[0], p1 = ml[1];
+            const float f0 = weight_of(p0.x, m[0]), f1 = weight_of(p0.z, m[1]), f2 = weight_of(p1.x, m[2]), f3 = weight_of(p1.z, m[3]);
+            l[0] = fmaf(f0, p0.y, l[0]); l[1] = fmaf(f1, p0.w, l[1]); l[2] = fmaf(f2, p1.y, l[2]); l[3] = fmaf(f3, p1.w, l[3]);
 #pragma unroll
-            for (int t = 0; t < kCombineTeams - 1; ++t) {
-                const float4 v = sums[t][x];
-                o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+            for (int g = 0; g < 4; ++g)
+                if (g < gn) {
+                    const float4 v = src[(size_t)place(k) * (kPartFloats / 4) + g * (2 * 8 * 32)];
+                    o[g].x = fmaf(f0, v.x, o[g].x); o[g].y = fmaf(f1, v.y, o[g].y); o[g].z = fmaf(f2, v.z, o[g].z); o[g].w = fmaf(f3, v.w, o[g].w);
+                }
+        }
+        if (!few) {
+            __shared__ float4 ls[kCombineThreads / 32];
+            sums[warp][0][lane] = o[0];
+            sums[warp][1][lane] = o[1];
+            if (lane == 0) ls[warp] = make_float4(l[0], l[1], l[2], l[3]);
+            __syncthreads();
+            if (warp == 0) {
+#pragma unroll 1
+                for (int y = 1; y < kCombineThreads / 32; ++y) {
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const float4 v = sums[y][g][lane];
+                        o[g].x += v.x; o[g].y += v.y; o[g].z += v.z; o[g].w += v.w;
+                    }
+                    const float4 v = ls[y];
+                    l[0] += v.x; l[1] += v.y; l[2] += v.z; l[3] += v.w;
+                }
             }
-            uint2 b;
-            b.x = pack2<T>(o.x, o.y);
-            b.y = pack2<T>(o.z, o.w);
-            *reinterpret_cast<uint2*>((T*)a.out + token * a.out_token + h * a.out_head + 4 * x) = b;
+            __syncthreads();
+            if (warp > 0) continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = row0 + e;
+            if (row < rows_all) {
+                const int j = a.by_heads(row), h = row - j * a.heads;
+                const long long token = (long long)own.x * a.q_len + j;
+                const float inv = l[e] == 0.f ? 0.f : rcp(l[e]);
+                T* out = (T*)a.out + token * a.out_token + h * a.out_head + 128 * g0 + 32 * w + lane;
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    if (g < gn) out[128 * g] = from_float<T>((e == 0 ? o[g].x : e == 1 ? o[g].y : e == 2 ? o[g].z : o[g].w) * inv);
+                if (w == 0 && g0 == 0 && lane == 0 && a.lse) a.lse[token * a.heads + h] = lse_of(m[e], l[e]);
+            }
         }
     }
 }
@@ -792,6 +936,13 @@ EncodeFn tensor_map_encoder() {
     return fn;
 }
 
+FastDiv fast_div(unsigned d, int bits) {
+    int log = 0;
+    while ((1u << log) < d) ++log;
+    const int shift = bits + log;
+    return FastDiv{(unsigned)(((1ull << shift) + d - 1) / d), (unsigned)shift};
+}
+
 constexpr size_t kOwnerBytes = kMaxGrid * sizeof(int4), kMlBytes = 2 * (size_t)kMaxGrid * kTileRows * sizeof(float2);
 constexpr size_t kAttWorkspace = kOwnerBytes + kMlBytes + 2 * (size_t)kMaxGrid * kPartFloats * sizeof(float);
 
@@ -804,7 +955,7 @@ int launch_attention(const CUtensorMap& map, const AttentionArgs& a, int grid, c
     }
     const int r = launch_latent(latent_attention_kernel<T>, dim3((unsigned)grid), kAttThreads, kAttSmem, st, map, a);
     if (r) return r;
-    return launch_latent(latent_combine_kernel<T>, dim3((unsigned)(4 * grid)), kCombineTeams * 128, 0, st, a, grid);
+    return launch_latent(latent_combine_kernel<T>, dim3((unsigned)(4 * sm_count())), kCombineThreads, 0, st, a, grid);
 }
 
 }  // namespace
@@ -847,18 +998,21 @@ extern "C" int vib3_launch_latent_attention_paged(const void* q, long long q_tok
     a.box_rows = page_size % 64 == 0 ? 64 : page_size % 32 == 0 ? 32 : page_size % 16 == 0 ? 16 : 8;
     a.page_table = page_table; a.table_stride = table_stride; a.max_pages = max_pages_per_seq;
     a.seq_lens = seq_lens; a.batch = batch; a.q_len = q_len; a.heads = heads;
+    a.by_heads = fast_div((unsigned)heads, 27);
+    a.by_page = fast_div((unsigned)page_size, 31);
     a.scale_log2 = scale * 1.4426950408889634074f;
     a.out = out; a.out_token = out_token_stride; a.out_head = out_head_stride;
     a.lse = lse_or_null; a.status = status;
     unsigned char* ws = static_cast<unsigned char*>(workspace);
     a.owner = reinterpret_cast<int4*>(ws);
     a.part_ml = reinterpret_cast<float2*>(ws + kOwnerBytes);
-    a.part_o = reinterpret_cast<float*>(ws + kOwnerBytes + kMlBytes);
+    a.part_o = reinterpret_cast<float4*>(ws + kOwnerBytes + kMlBytes);
     const int blocks = (int)(((long long)q_len * heads + kTileRows - 1) / kTileRows);
     const int sms = sm_count() < kMaxGrid ? sm_count() : kMaxGrid;
     a.lanes = blocks <= 8 ? blocks : 1;
     a.blocks_per_lane = blocks / a.lanes;
-    if ((long long)batch * a.blocks_per_lane > 0x7fffffff) return VIB3_ERR_COUNT;
+    // the kernel counts tiles in 32 bits
+    if ((long long)batch * a.blocks_per_lane * (((long long)max_pages_per_seq * page_size + kTileKeys - 1) / kTileKeys) > 0x7fffffff) return VIB3_ERR_COUNT;
     a.min_tiles = 2;
     const int grid = sms / a.lanes * a.lanes;
 
