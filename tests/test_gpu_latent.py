@@ -376,3 +376,13 @@ def test_a_step_on_a_side_stream_and_in_a_graph_with_new_lengths(cuda_dev):
         feed(i)
         graph.replay()
         verify()
+
+
+@pytest.mark.parametrize("lens,q_len,heads", [
+    ([0, 0, 0], 1, 64), ([0] * 40 + [64] * 3 + [0] * 50 + [1], 1, 8), ([64, 0, 128, 0, 0, 64] * 30, 1, 64), ([1, 0] * 300, 1, 4),
+    ([192, 0, 0, 64 * 37, 0], 2, 40), ([0, 5] * 20, 70, 16), ([64] * 148, 1, 64), ([128] * 149 + [0], 1, 64)])
+def test_attention_with_sequences_of_no_tokens_between_others(cuda_dev, lens, q_len, heads):
+    """Empty sequences stand at the borders of the CTAs' shares too: each of their rows is written by somebody."""
+    cache, table, lens = paged(cuda_dev, lens, 64, torch.bfloat16, 21)
+    q = torch.randn(lens.numel() * q_len, heads, ROW, generator=gen(cuda_dev, 22), device=cuda_dev).to(torch.bfloat16)
+    check_attention(q, cache, table, lens, 0.07)

@@ -67,10 +67,12 @@ struct AttentionArgs {
     long long out_token, out_head;
     float* lse;
     int* status;
+    int block_rows;                        // rows of a row block: kTileRows, or half of them
     int lanes, blocks_per_lane;            // see Plan
-    int min_tiles;
-    // workspace: what CTA c owes to a sequence that other CTAs share, two slots per CTA
-    int4* owner;                           // [grid] sequence, row block, parts (0: none)
+    int min_cost;                          // of a share
+    // workspace: what a sequence's row block is made of, and two places per CTA for parts
+    int4* made_of;                         // [items or grid] sequence, row block, parts (fewer than 2: nothing to add up), first CTA
+    int by_item;                           // whether made_of goes by item or by the CTA that begins it
     float2* part_ml;                       // [2 grid][64] reference (log2) and sum
     float4* part_o;                        // [2 grid][4][8][8][32] x 4 rows: 64 x 512 values, not yet divided by the sum
 };
@@ -86,19 +88,24 @@ struct Plan {
 };
 
 struct Piece {
-    int b, rb, seen, tiles;                // item: sequence, row block, keys of its last row, tiles
+    int b, rb, len, seen, tiles;           // item: sequence, row block, keys of the sequence and of the block's last row, tiles
     int t0, t1;                            // this CTA's tiles of it
     int prefix;
 };
+
+// A row block costs what its tiles do and kPieceCost more (Q, the results, filling the pipe: 8000 to 10000 cycles), so on the line it begins
+// with a stretch without tiles.  (Without it a CTA with the ends of several short sequences took twice the average.)
+constexpr int kPieceCost = 3, kMinCost = 2;
+__device__ __forceinline__ int cost_of(const Piece& p) { return p.tiles ? p.tiles + kPieceCost : 0; }
 
 __device__ __forceinline__ int first_tile(const Plan& p, int share) { return share * p.per + min(share, p.rem); }
 
 __device__ __forceinline__ void item_of(const AttentionArgs& a, int b, int rb, Piece& p) {
     p.b = b;
     p.rb = rb;
-    const int last_row = min(a.q_len * a.heads, (rb + 1) * kTileRows) - 1;
-    const int len = max(__ldg(a.seq_lens + b), 0);
-    p.seen = min(max(len - a.q_len + a.by_heads(last_row) + 1, 0), a.max_pages * a.page_size);
+    const int last_row = min(a.q_len * a.heads, (rb + 1) * a.block_rows) - 1;
+    p.len = max(__ldg(a.seq_lens + b), 0);
+    p.seen = min(max(p.len - a.q_len + a.by_heads(last_row) + 1, 0), a.max_pages * a.page_size);
     p.tiles = (p.seen + kTileKeys - 1) / kTileKeys;
 }
 
@@ -118,9 +125,9 @@ struct Walk {
                 ++b;
             }
             p.prefix = prefix;
-            prefix += p.tiles;
-            p.t0 = max(begin - p.prefix, 0);
-            p.t1 = min(end - p.prefix, p.tiles);
+            prefix += cost_of(p);
+            p.t0 = max(begin - p.prefix - kPieceCost, 0);
+            p.t1 = min(end - p.prefix - kPieceCost, p.tiles);
             if (p.tiles == 0 ? empty : !empty && p.t1 > p.t0) return true;
         }
         return false;
@@ -134,8 +141,6 @@ struct AttShared {
     alignas(16) float factor[kTileRows];
     float team[2][kTileRows];              // what the two softmax teams have of a row: maximum, sum
     alignas(16) float inv[kTileRows];
-    Plan plan;
-    int warp_sum[kAttThreads / 32];
     uint32_t tmem;
 };
 static_assert(kMiscOff + sizeof(AttShared) <= 227 * 1024, "shared memory of a CTA");
@@ -261,87 +266,67 @@ __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t* r) {
                  : "r"(taddr) : "memory");
 }
 
+__device__ __forceinline__ void tmem_st_16x32(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
 
-// This CTA's place on its lane's line of tiles.  All threads.  (The line has fewer than 2^31 tiles: checked by the launcher.)
-__device__ __forceinline__ void make_plan(const AttentionArgs& a, AttShared& sh) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// This CTA's place on its lane's line of tiles, by every warp for itself: a lane sums the tiles of a run of items, the runs are added up, and the
+// lane whose run has the place finds the item.  (The line has fewer than 2^31 tiles: checked by the launcher.)
+__device__ __forceinline__ Plan make_plan(const AttentionArgs& a) {
+    const int lane = threadIdx.x & 31;
     const int row_lane = a.lanes == 1 ? 0 : blockIdx.x % a.lanes, share = a.lanes == 1 ? blockIdx.x : blockIdx.x / a.lanes;
     const int most = a.lanes == 1 ? gridDim.x : gridDim.x / a.lanes, items = a.batch * a.blocks_per_lane;
+    const int run = (items + 31) >> 5, i0 = min(lane * run, items), i1 = min(i0 + run, items);
+    const int b0 = a.blocks_per_lane == 1 ? i0 : i0 / a.blocks_per_lane, rb_first = row_lane * a.blocks_per_lane;
     Piece p;
-    p.tiles = p.b = p.rb = 0;
-    auto look = [&](int i) {
-        const int b = a.blocks_per_lane == 1 ? i : i / a.blocks_per_lane;
-        item_of(a, b, row_lane * a.blocks_per_lane + i - b * a.blocks_per_lane, p);
-    };
-    // Pass 0 sums the tiles of all items, pass 1 finds the first item that begins at `begin` or reaches beyond it; a single chunk of
-    // items (the usual batch) needs no second look at the lengths.
-    int total = 0, begin = 0, end = 0, base = 0, pass = 0;
-#pragma unroll 1
-    for (int i0 = 0;;) {
-        const int i = i0 + tid;
-        if (i < items) look(i);
-        else p.tiles = 0;
-        int incl = p.tiles;
-#pragma unroll
-        for (int m = 1; m < 32; m <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, incl, m);
-            if (lane >= m) incl += o;
+    int sum = 0;
+    for (int i = i0, b = b0, x = i0 - b0 * a.blocks_per_lane; i < i1; ++i) {
+        item_of(a, b, rb_first + x, p);
+        sum += cost_of(p);
+        if (++x == a.blocks_per_lane) {
+            x = 0;
+            ++b;
         }
-        __syncthreads();
-        if (lane == 31) sh.warp_sum[warp] = incl;
-        __syncthreads();
-        int before = 0, chunk = 0;
-#pragma unroll 1
-        for (int w = 0; w < kAttThreads / 32; ++w) {
-            if (w == warp) before = chunk;
-            chunk += sh.warp_sum[w];
-        }
-        if (pass == 0) {
-            total += chunk;
-            if (i0 + kAttThreads < items) {
-                i0 += kAttThreads;
-                continue;
-            }
-            const int shares = max(1, min(most, (total + a.min_tiles - 1) / a.min_tiles));
-            const int per = total / shares, rem = total - per * shares;
-            begin = share * per + min(share, rem);
-            end = begin + per + (share < rem);
-            if (tid == 0) {
-                sh.plan.begin = begin; sh.plan.end = end; sh.plan.prefix = 0;
-                sh.plan.b = a.batch; sh.plan.rb = 0;      // (nothing, unless an item is found below)
-                sh.plan.share = share; sh.plan.shares = shares; sh.plan.per = per; sh.plan.rem = rem;
-            }
-            if (share >= shares) return;
-            pass = 1;
-            __syncthreads();
-            if (items > kAttThreads) {
-                i0 = 0;
-                continue;
-            }
-        }
-        const int pre = base + before + incl - p.tiles;
-        // of those that qualify the first one: with the beginning in common only items without tiles come before it
-        if (i < items && pre <= begin && (pre == begin || pre + p.tiles > begin)) {
-            const int b = p.b, rb = p.rb;
-            bool first = true;
-            if (pre == begin && i > 0) {
-                look(i - 1);
-                first = p.tiles > 0;
-            }
-            if (first) {
-                sh.plan.b = b;
-                sh.plan.rb = rb;
-                sh.plan.prefix = pre;
-            }
-        }
-        base += chunk;
-        i0 += kAttThreads;
-        if (base > begin || i0 >= items) break;
     }
+    int incl = sum;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, m);
+        if (lane >= m) incl += o;
+    }
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    const int shares = max(1, min(most, (total + a.min_cost - 1) / a.min_cost));
+    const int per = total / shares, rem = total - per * shares;
+    const int begin = share * per + min(share, rem), end = begin + per + (share < rem);
+    // the first item that begins at `begin` (items without tiles among them) or reaches beyond it
+    int prefix = incl - sum, b = b0, x = i0 - b0 * a.blocks_per_lane;
+    bool found = false;
+    if (share < shares && i0 < i1 && prefix <= begin && incl >= begin) {
+#pragma unroll 1
+        for (int i = i0; i < i1; ++i) {
+            item_of(a, b, rb_first + x, p);
+            found = prefix == begin || prefix + cost_of(p) > begin;
+            if (found) break;
+            prefix += cost_of(p);
+            if (++x == a.blocks_per_lane) {
+                x = 0;
+                ++b;
+            }
+        }
+    }
+    const unsigned hits = __ballot_sync(0xffffffffu, found);
+    const int who = hits ? __ffs(hits) - 1 : 0;      // (the first lane: a later one may begin at the same place)
+    Plan plan;
+    plan.begin = begin; plan.end = end; plan.share = share; plan.shares = shares; plan.per = per; plan.rem = rem;
+    plan.prefix = __shfl_sync(0xffffffffu, prefix, who);
+    plan.b = hits ? __shfl_sync(0xffffffffu, b, who) : a.batch;      // nothing for a CTA beyond the shares
+    plan.rb = __shfl_sync(0xffffffffu, rb_first + x, who);
+    return plan;
 }
 
 template <typename T>
@@ -371,16 +356,22 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (warp == 0 && elect_one()) asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
-    pdl_enter();
-    make_plan(a, sh);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = uniform(sh.tmem);
-    const Plan& plan = sh.plan;
+    pdl_wait_only();
+    const Plan plan = make_plan(a);
+    // The copying warp set the barriers up itself and need not wait for the others.
+    uint32_t tmem = 0;
+    if (warp == 0) {
+        __syncwarp();
+        asm volatile("bar.arrive 2, %0;" ::"n"(kAttThreads) : "memory");
+    } else {
+        tc_fence_before();
+        asm volatile("bar.sync 2, %0;" ::"n"(kAttThreads) : "memory");
+        tc_fence_after();
+        tmem = uniform(sh.tmem);
+    }
     const int rows_all = a.q_len * a.heads;
     Walk walk(a, plan, a.lanes == 1 ? 0 : (int)(blockIdx.x % a.lanes) * a.blocks_per_lane);
-    Piece p;
+    Piece p = {};
     bool ok = (base & 1023) == 0;   // the swizzle is a function of the address
     // tile `it` of this CTA: its latent chunk pairs lie in ring slots 4 it .. 4 it + 3 (mod kSlots), its position values in place it mod kTiles
     int it = 0, slot = 0, place = 0;
@@ -412,9 +403,13 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
                 const int page = __shfl_sync(0xffffffffu, page_of, src), key = key0 + lane * R;
                 const bool mine = lane < nb, live = mine && key < p.seen, good = live && page >= 0 && page < a.num_pages;
                 if (live && !good && a.status) atomicOr(a.status, kStatusBadPage);
-                const unsigned long long bits = (good ? (R == 64 ? ~0ull : (1ull << R) - 1) << (lane * R & 63) : 0ull);
-                unsigned long long m = (unsigned long long)__reduce_or_sync(0xffffffffu, (unsigned)(bits >> 32)) << 32 |
-                                       __reduce_or_sync(0xffffffffu, (unsigned)bits);
+                const unsigned boxes = __ballot_sync(0xffffffffu, good);
+                unsigned long long m = ~0ull;
+                if (boxes != (nb == 8 ? 0xffu : (1u << nb) - 1)) {
+                    m = 0;
+                    for (int x = 0; x < nb; ++x)
+                        if (boxes >> x & 1) m |= (R == 64 ? ~0ull : (1ull << R) - 1) << (x * R);
+                }
                 if (p.seen - key0 < 64) m &= (1ull << (p.seen - key0)) - 1;
                 const int y = key - a.by_page(key) * a.page_size, z = good ? page : a.num_pages;   // z = num_pages: outside, read as zeros
                 const uint32_t row = lane * R * 128;
@@ -530,8 +525,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
         // ── Q of the later pieces into L2: fetched from HBM under the streaming tiles it took 5000 cycles between two pieces ──
         for (bool first = true; ok && walk.next(p, false); first = false) {
             if (first) continue;
-            for (int r = lane; r < kTileRows; r += 32) {
-                const int row = p.rb * kTileRows + r, j = a.by_heads(row);
+            for (int r = lane; r < a.block_rows; r += 32) {
+                const int row = p.rb * a.block_rows + r, j = a.by_heads(row);
                 if (row >= rows_all) break;
                 const T* q = (const T*)a.q + ((long long)p.b * a.q_len + j) * a.q_token + (row - j * a.heads) * a.q_head;
 #pragma unroll
@@ -547,40 +542,51 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
         const int stid = tid - 128;
         // Q of a piece (behind its last row that row again: what comes of it is not stored): six chunks of its nine to tensor memory (row 16 w + i is lane 32 w + i, two
         // values per column), three to shared memory.  Its place is free: the scores of the piece before have been seen.
-        auto load_q = [&](const Piece& n) {
+        // (In the order of the 16 x 256-bit store a load of the warp takes 32 bytes of eight rows; with a row per lane it touched 16 lines
+        // for 16 bytes each, and Q took 6900 cycles, the table entry behind it 4700.)
+        uint2 qv[3][4][2];
+        auto fetch_q = [&](const Piece& n) {
             const T* q = (const T*)a.q + (long long)n.b * a.q_len * a.q_token;
             auto row_at = [&](int r) {
-                const int row = min(n.rb * kTileRows + r, rows_all - 1), j = a.by_heads(row);
+                const int row = min(n.rb * a.block_rows + r, rows_all - 1), j = a.by_heads(row);
                 return q + j * a.q_token + (row - j * a.heads) * a.q_head;
             };
-            const T* src = row_at(16 * w + (lane & 15)) + 3 * team * 64;
-            uint4 v[3][8];
+            const T *src0 = row_at(r0) + 3 * team * 64 + 4 * (lane & 3), *src1 = row_at(r1) + 3 * team * 64 + 4 * (lane & 3);
 #pragma unroll
             for (int c = 0; c < 3; ++c)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[c][i] = __ldg(reinterpret_cast<const uint4*>(src + c * 64 + i * 8));
+                for (int i = 0; i < 4; ++i) {
+                    qv[c][i][0] = __ldg(reinterpret_cast<const uint2*>(src0 + c * 64 + i * 16));
+                    qv[c][i][1] = __ldg(reinterpret_cast<const uint2*>(src1 + c * 64 + i * 16));
+                }
             if (lane < 24) {
                 const uint32_t dst = base + kQOff + (lane >> 3) * kChunkBytes + 8 * (warp - 4) * 128;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) cp_async16(dst + i * 128 + (((lane & 7) ^ i) << 4), row_at(8 * (warp - 4) + i) + kQTmemChunks * 64 + lane * 8);
             }
+        };
+        auto store_q = [&] {
 #pragma unroll
-            for (int c = 0; c < 3; ++c) tmem_st_32x32(tmem + kQCol + 32 * (3 * team + c) + quarter, reinterpret_cast<const uint32_t*>(v[c]));
+            for (int c = 0; c < 3; ++c) tmem_st_16x32(tmem + kQCol + 32 * (3 * team + c) + quarter, reinterpret_cast<const uint32_t*>(qv[c]));
             tmem_st_wait();
             asm volatile("cp.async.wait_all;" ::: "memory");
             proxy_fence();
             tc_fence_before();
             bar_arrive(&sh.q_full);
         };
-        if (stid == 0) a.owner[blockIdx.x] = make_int4(0, 0, 0, 0);
-        // A round: the next piece's Q (under the last product of the piece before), that piece's results, the next one's tiles.
+        if (stid == 0 && !a.by_item) a.made_of[blockIdx.x] = make_int4(0, 0, 0, 0);
+        // A round: the next piece's Q requested, the results of the piece before, with Q put in place half way, the next one's tiles.
         float m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f;
         long long token0 = 0;
         Piece next;
 #pragma unroll 1
         for (bool open = false; open || ok; open = true) {
             const bool more = walk.next(next, false);
-            if (more) load_q(next);
+            if (more) fetch_q(next);
+            // The adding launch may come now.  (Earlier its blocks crowd on the SMs that have no CTA of this one, and the others stay idle.)
+            else if (stid == 0) pdl_release();
+            const bool whole = open && p.t0 == 0 && p.t1 == p.tiles;
+            const int part = 2 * blockIdx.x + (p.t0 == 0 ? 1 : 0);
             if (open) {
                 ok = ok && bar_wait(&sh.pv_done[(it - 1) & 1], (unsigned)((it - 1) >> 1) & 1);
                 ok = !softmax_any(!ok);
@@ -596,78 +602,73 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
                     sh.team[1][r1] = l1;
                 }
                 softmax_sync();
-                const bool whole = p.t0 == 0 && p.t1 == p.tiles;
-                const int part = 2 * blockIdx.x + (p.t0 == 0 ? 1 : 0);
                 if (team == 0 && (lane & 3) == 0) {
-                    const int row0 = p.rb * kTileRows + r0, row1 = row0 + 8;
+                    const int row0 = p.rb * a.block_rows + r0, row1 = row0 + 8;
                     l0 += sh.team[1][r0];
                     l1 += sh.team[1][r1];
                     if (whole) {
                         sh.inv[r0] = l0 == 0.f ? 0.f : rcp(l0);
                         sh.inv[r1] = l1 == 0.f ? 0.f : rcp(l1);
                         if (a.lse) {
-                            if (row0 < rows_all) a.lse[token0 * a.heads + row0] = lse_of(m0, l0);
-                            if (row1 < rows_all) a.lse[token0 * a.heads + row1] = lse_of(m1, l1);
+                            if (r0 < a.block_rows && row0 < rows_all) a.lse[token0 * a.heads + row0] = lse_of(m0, l0);
+                            if (r1 < a.block_rows && row1 < rows_all) a.lse[token0 * a.heads + row1] = lse_of(m1, l1);
                         }
                     } else {
                         a.part_ml[part * kTileRows + r0] = make_float2(m0, l0);
                         a.part_ml[part * kTileRows + r1] = make_float2(m1, l1);
                     }
                 }
-                if (!whole && p.t0 == 0 && stid == 0) {
-                    // the share that holds the item's last tile
-                    const int x = p.prefix + p.tiles - 1, wide = plan.rem * (plan.per + 1);
-                    const int last = x < wide ? x / (plan.per + 1) : plan.rem + (x - wide) / plan.per;
-                    a.owner[blockIdx.x] = make_int4(p.b, p.rb, last - plan.share + 1, 0);
+                if (p.t0 == 0 && stid == 0 && (a.by_item || !whole)) {
+                    // up to the share that holds the item's last tile
+                    const int x = p.prefix + kPieceCost + p.tiles - 1, wide = plan.rem * (plan.per + 1);
+                    const int last = whole ? plan.share : x < wide ? x / (plan.per + 1) : plan.rem + (x - wide) / plan.per;
+                    a.made_of[a.by_item ? p.b * a.lanes * a.blocks_per_lane + p.rb : (int)blockIdx.x] = make_int4(p.b, p.rb, last - plan.share + 1, blockIdx.x);
                 }
-                if (whole) {
-                    softmax_sync();
-                    const int n = min(kTileRows, rows_all - p.rb * kTileRows), sub = lane & 3;
+                if (whole) softmax_sync();
+            }
+            const int n = min(a.block_rows, rows_all - p.rb * a.block_rows), sub = lane & 3;
+            // O's columns 32 x ..: rows 32 (x & 1) .. of the values 128 (x >> 1) + 32 w + lane; a team has half of them
 #pragma unroll 1
-                    for (int x = 4 * team; x < 4 * team + 4; ++x) {
-                        uint32_t o[32];
-                        tmem_ld_32x32(tmem + 32 * x + quarter, o);
-                        tmem_ld_wait();
-                        // a lane has one value of 32 rows; four lanes exchange theirs, so that each has four neighbouring values of eight rows
-                        transpose4(o, sub);
-                        int r = 32 * (x & 1) + sub;
-                        T* out = (T*)a.out + token0 * a.out_token + 128 * (x >> 1) + 32 * w + (lane & ~3);
+            for (int y = 0; y < 4; y += a.block_rows > 32 ? 1 : 2) {
+                if (y == 2 && more) store_q();
+                if (!open) continue;
+                const int x = 4 * team + y;
+                uint32_t o[32];
+                tmem_ld_32x32(tmem + 32 * x + quarter, o);
+                tmem_ld_wait();
+                if (whole) {
+                    // a lane has one value of 32 rows; four lanes exchange theirs, so that each has four neighbouring values of eight rows
+                    transpose4(o, sub);
+                    int r = 32 * (x & 1) + sub;
+                    T* out = (T*)a.out + token0 * a.out_token + 128 * (x >> 1) + 32 * w + (lane & ~3);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i, r += 4) {
-                            if (r < n) {
-                                const int row = p.rb * kTileRows + r, j = a.by_heads(row), h = row - j * a.heads;
-                                const float f = sh.inv[r];
-                                uint2 b;
-                                b.x = pack2<T>(__uint_as_float(o[4 * i]) * f, __uint_as_float(o[4 * i + 1]) * f);
-                                b.y = pack2<T>(__uint_as_float(o[4 * i + 2]) * f, __uint_as_float(o[4 * i + 3]) * f);
-                                *reinterpret_cast<uint2*>(out + j * a.out_token + h * a.out_head) = b;
-                            }
+                    for (int i = 0; i < 8; ++i, r += 4) {
+                        if (r < n) {
+                            const int row = p.rb * a.block_rows + r, j = a.by_heads(row), h = row - j * a.heads;
+                            const float f = sh.inv[r];
+                            uint2 b;
+                            b.x = pack2<T>(__uint_as_float(o[4 * i]) * f, __uint_as_float(o[4 * i + 1]) * f);
+                            b.y = pack2<T>(__uint_as_float(o[4 * i + 2]) * f, __uint_as_float(o[4 * i + 3]) * f);
+                            *reinterpret_cast<uint2*>(out + j * a.out_token + h * a.out_head) = b;
                         }
                     }
                 } else {
                     // in the order in which the values lie in registers: four rows of a value are 16 bytes, a warp's 32 values 512
                     float4* out = a.part_o + (size_t)part * (kPartFloats / 4) + w * (8 * 8 * 32) + lane;
-#pragma unroll 1
-                    for (int x = 4 * team; x < 4 * team + 4; ++x) {
-                        uint32_t o[32];
-                        tmem_ld_32x32(tmem + 32 * x + quarter, o);
-                        tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            out[(x * 8 + i) * 32] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
-                                                                __uint_as_float(o[4 * i + 3]));
-                    }
+                    for (int i = 0; i < 8; ++i)
+                        out[(x * 8 + i) * 32] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                                                            __uint_as_float(o[4 * i + 3]));
                 }
-                tc_fence_before();
             }
+            tc_fence_before();
             if (!more) break;
             p = next;
-            const int len = max(__ldg(a.seq_lens + p.b), 0);
             token0 = (long long)p.b * a.q_len;
-            if (stid == 0 && len > a.max_pages * a.page_size && a.status) atomicOr(a.status, kStatusBadPage);
-            const int j0 = a.by_heads(p.rb * kTileRows + r0), j1 = a.by_heads(p.rb * kTileRows + r1);
-            const int seen0 = min(len - a.q_len + j0 + 1, p.seen), seen1 = min(len - a.q_len + j1 + 1, p.seen);
-            const int seen_all = min(len - a.q_len + a.by_heads(p.rb * kTileRows) + 1, p.seen);    // keys that every row sees
+            if (stid == 0 && p.len > a.max_pages * a.page_size && a.status) atomicOr(a.status, kStatusBadPage);
+            const int j0 = a.by_heads(p.rb * a.block_rows + r0), j1 = a.by_heads(p.rb * a.block_rows + r1);
+            const int seen0 = min(p.len - a.q_len + j0 + 1, p.seen), seen1 = min(p.len - a.q_len + j1 + 1, p.seen);
+            const int seen_all = min(p.len - a.q_len + a.by_heads(p.rb * a.block_rows) + 1, p.seen);    // keys that every row sees
             m0 = m1 = -INFINITY;
             l0 = l1 = 0.f;
 #pragma unroll 1
@@ -742,7 +743,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
                         __syncwarp();
                         tc_fence_after();
 #pragma unroll 1
-                        for (int x = 4 * team; x < 4 * team + 4; ++x) {
+                        for (int x = 4 * team; x < 4 * team + 4; x += a.block_rows > 32 ? 1 : 2) {
                             uint32_t o[32];
                             tmem_ld_32x32(tmem + 32 * x + quarter, o);
                             tmem_ld_wait();
@@ -790,9 +791,10 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
         // Items of this CTA that have no tiles: no row of theirs sees a key.
         Walk none(a, plan, walk.rb0);
         while (ok && none.next(p, true)) {
-            const int n = min(kTileRows, rows_all - p.rb * kTileRows);
+            const int n = min(a.block_rows, rows_all - p.rb * a.block_rows);
+            if (stid == 0 && a.by_item) a.made_of[p.b * a.lanes * a.blocks_per_lane + p.rb] = make_int4(0, 0, 0, 0);
             for (int r = warp - 4; r < n; r += 8) {
-                const int row = p.rb * kTileRows + r, j = a.by_heads(row), h = row - j * a.heads;
+                const int row = p.rb * a.block_rows + r, j = a.by_heads(row), h = row - j * a.heads;
                 const long long token = (long long)p.b * a.q_len + j;
                 uint4* o = reinterpret_cast<uint4*>((T*)a.out + token * a.out_token + h * a.out_head);
                 o[lane] = o[lane + 32] = make_uint4(0, 0, 0, 0);
@@ -800,6 +802,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
             }
         }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (!ok && lane == 0 && a.status) atomicOr(a.status, 4 /* VIB3_STATUS_TIMEOUT */);
     tc_fence_before();
     __syncthreads();
@@ -809,113 +812,103 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
     }
 }
 
-// Adds up the parts of the sequences that several CTAs shared.  Parts of an owner c lie in its second place and in the first places of
-// the CTAs after it in its lane.  Every block lists the owners; a warp's work is four rows and 128 of the 512 values (of a part, each
-// value's four rows are 16 bytes).  With few parts it adds all of them; with many, a block's eight warps take every eighth part of the same
-// four rows and half of those values, and meet in shared memory.  It works out its rows' weights itself, so that nothing waits for
-// other warps.  (Both ways are needed: a warp for all parts took 100 us where one sequence had 148, a block per row 35 us where 128 sequences had two.)
-constexpr int kCombineFew = 8, kCombineThreads = 256;
+// Adds up the parts of the row blocks that several CTAs shared.  The parts lie in the second place of the CTA that begins the block and in
+// the first places of the CTAs after it in its lane.  A unit of work is four rows and 32 of every 128 values (all four 128s, or two of
+// them).  One warp adds up to four parts of a unit; of more parts `team` warps take every team-th each and meet in shared memory.
+// How large a team, and with it the grid, the launcher chooses by the number of row blocks: a few may have up to 148 parts each,
+// many have about two, and then the blocks beyond the first return at once.
+constexpr int kCombineThreads = 256, kCombineWarps = kCombineThreads / 32, kCombineAlone = 4;
 
-template <typename T>
-__global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const AttentionArgs a, int grid) {
-    __shared__ int4 owners[kMaxGrid];
-    __shared__ int upto[kCombineThreads];      // blocks of work up to and with owner c
-    __shared__ int warp_sum[kCombineThreads / 32];
-    __shared__ float4 sums[kCombineThreads / 32][2][32];
+template <typename T, int GN>
+__global__ void __launch_bounds__(kCombineThreads, 2) latent_combine_kernel(const AttentionArgs a, int most) {
+    constexpr int kHalves = 4 / GN, kDepth = 8 / GN;     // parts whose loads are in flight together
+    __shared__ float4 sums[kCombineWarps][GN][32];
+    __shared__ float4 weights[kCombineWarps];
     pdl_enter();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rows_all = a.q_len * a.heads;
-    int units = 0;
-    if (tid < grid) {
-        const int4 own = a.owner[tid];
-        owners[tid] = own;
-        units = own.z == 0 ? 0 : own.z <= kCombineFew ? 8 : 128;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows_all = a.q_len * a.heads;
+    const int4 own = a.made_of[blockIdx.y];
+    const int parts = own.z, c = own.w, team = parts <= kCombineAlone ? 1 : most;
+    const int x = blockIdx.x * kCombineWarps + warp, mate = x & (team - 1), unit = x / team;
+    if (parts < 2 || unit >= a.block_rows * kHalves) return;      // (the same for all warps of a block: team divides their number)
+    const int half = unit % kHalves, u = unit / kHalves;
+    // rows r .. r + 3 of the block, values 128 g + 32 w + lane with g in [g0, g0 + GN)
+    const int w = u & 3, r = (u >> 2) * 4, g0 = GN * half, row0 = own.y * a.block_rows + r;
+    auto place = [&](int k) { return 2 * (c + k * a.lanes) + (k == 0); };
+    const float4* src = a.part_o + (w * 64 + (2 * g0 + (r >> 5)) * 8 + ((r & 31) >> 2)) * 32 + lane;
+    const float4* ml = reinterpret_cast<const float4*>(a.part_ml + r);     // (m, l) of two rows each
+    constexpr int kMl = kTileRows / 2;
+    float4 v[kDepth][GN];
+    auto fetch = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < kDepth; ++i)
+#pragma unroll
+            for (int g = 0; g < GN; ++g) v[i][g] = src[(size_t)place(min(k + i * team, parts - 1)) * (kPartFloats / 4) + g * (2 * 8 * 32)];
+    };
+    fetch(mate);
+    float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll 1
+    for (int k = lane; k < parts; k += 32) {
+        const float4 p = ml[place(k) * kMl], q = ml[place(k) * kMl + 1];
+        m0 = fmaxf(m0, p.x); m1 = fmaxf(m1, p.z); m2 = fmaxf(m2, q.x); m3 = fmaxf(m3, q.z);
     }
 #pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, units, m);
-        if (lane >= m) units += o;
+    for (int y = 16; y; y >>= 1) {
+        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, y)); m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, y));
+        m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, y)); m3 = fmaxf(m3, __shfl_xor_sync(0xffffffffu, m3, y));
     }
-    if (lane == 31) warp_sum[warp] = units;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) units += warp_sum[w];
-    upto[tid] = units;
-    __syncthreads();
-    const int all = upto[kCombineThreads - 1];
+    float4 o[GN], l = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int g = 0; g < GN; ++g) o[g] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-    for (int u = blockIdx.x; u < all; u += gridDim.x) {
-        int c = 0;
+    for (int k = mate; k < parts; k += kDepth * team) {
+        if (k != mate) fetch(k);
 #pragma unroll
-        for (int step = kCombineThreads / 2; step; step >>= 1) c += upto[c + step - 1] <= u ? step : 0;
-        const int4 own = owners[c];
-        const int parts = own.z, x = u - (c ? upto[c - 1] : 0);
-        const bool few = parts <= kCombineFew;
-        // rows r .. r + 3 (of the block's 64), values 128 g + 32 w + lane with g in [g0, g0 + gn)
-        const int r = few ? (x * 2 + (warp >> 2)) * 4 : (x >> 3) * 4, w = few ? warp & 3 : (x >> 1) & 3, g0 = few ? 0 : 2 * (x & 1), gn = few ? 4 : 2;
-        const int row0 = own.y * kTileRows + r;
-        if (few && row0 >= rows_all) continue;     // (of the other kind all warps come to the barriers below)
-        auto place = [&](int k) { return 2 * (c + k * a.lanes) + (k == 0); };
-        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, l[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-        for (int k = lane; k < parts; k += 32)
+        for (int i = 0; i < kDepth; ++i) {
+            const int ki = k + i * team;
+            if (ki < parts) {
+                const float4 p = ml[place(ki) * kMl], q = ml[place(ki) * kMl + 1];
+                const float f0 = weight_of(p.x, m0), f1 = weight_of(p.z, m1), f2 = weight_of(q.x, m2), f3 = weight_of(q.z, m3);
+                l.x = fmaf(f0, p.y, l.x); l.y = fmaf(f1, p.w, l.y); l.z = fmaf(f2, q.y, l.z); l.w = fmaf(f3, q.w, l.w);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], a.part_ml[place(k) * kTileRows + r + e].x);
-#pragma unroll
-        for (int y = 16; y; y >>= 1)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], y));
-        float4 o[4];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) o[g] = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4* src = a.part_o + (w * 64 + (2 * g0 + (r >> 5)) * 8 + ((r & 31) >> 2)) * 32 + lane;
-#pragma unroll 4
-        for (int k = few ? 0 : warp; k < parts; k += few ? 1 : kCombineThreads / 32) {
-            const float4* ml = reinterpret_cast<const float4*>(a.part_ml + place(k) * kTileRows + r);
-            const float4 p0 = ml[0], p1 = ml[1];
-            const float f0 = weight_of(p0.x, m[0]), f1 = weight_of(p0.z, m[1]), f2 = weight_of(p1.x, m[2]), f3 = weight_of(p1.z, m[3]);
-            l[0] = fmaf(f0, p0.y, l[0]); l[1] = fmaf(f1, p0.w, l[1]); l[2] = fmaf(f2, p1.y, l[2]); l[3] = fmaf(f3, p1.w, l[3]);
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-                if (g < gn) {
-                    const float4 v = src[(size_t)place(k) * (kPartFloats / 4) + g * (2 * 8 * 32)];
-                    o[g].x = fmaf(f0, v.x, o[g].x); o[g].y = fmaf(f1, v.y, o[g].y); o[g].z = fmaf(f2, v.z, o[g].z); o[g].w = fmaf(f3, v.w, o[g].w);
-                }
-        }
-        if (!few) {
-            __shared__ float4 ls[kCombineThreads / 32];
-            sums[warp][0][lane] = o[0];
-            sums[warp][1][lane] = o[1];
-            if (lane == 0) ls[warp] = make_float4(l[0], l[1], l[2], l[3]);
-            __syncthreads();
-            if (warp == 0) {
-#pragma unroll 1
-                for (int y = 1; y < kCombineThreads / 32; ++y) {
-#pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const float4 v = sums[y][g][lane];
-                        o[g].x += v.x; o[g].y += v.y; o[g].z += v.z; o[g].w += v.w;
-                    }
-                    const float4 v = ls[y];
-                    l[0] += v.x; l[1] += v.y; l[2] += v.z; l[3] += v.w;
+                for (int g = 0; g < GN; ++g) {
+                    o[g].x = fmaf(f0, v[i][g].x, o[g].x); o[g].y = fmaf(f1, v[i][g].y, o[g].y);
+                    o[g].z = fmaf(f2, v[i][g].z, o[g].z); o[g].w = fmaf(f3, v[i][g].w, o[g].w);
                 }
             }
-            __syncthreads();
-            if (warp > 0) continue;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int row = row0 + e;
-            if (row < rows_all) {
-                const int j = a.by_heads(row), h = row - j * a.heads;
-                const long long token = (long long)own.x * a.q_len + j;
-                const float inv = l[e] == 0.f ? 0.f : rcp(l[e]);
-                T* out = (T*)a.out + token * a.out_token + h * a.out_head + 128 * g0 + 32 * w + lane;
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    if (g < gn) out[128 * g] = from_float<T>((e == 0 ? o[g].x : e == 1 ? o[g].y : e == 2 ? o[g].z : o[g].w) * inv);
-                if (w == 0 && g0 == 0 && lane == 0 && a.lse) a.lse[token * a.heads + h] = lse_of(m[e], l[e]);
-            }
         }
     }
+    if (team > 1) {
+#pragma unroll
+        for (int g = 0; g < GN; ++g) sums[warp][g][lane] = o[g];
+        if (lane == 0) weights[warp] = l;
+        __syncthreads();
+        if (mate > 0) return;
+#pragma unroll 1
+        for (int y = 1; y < team; ++y) {
+#pragma unroll
+            for (int g = 0; g < GN; ++g) {
+                const float4 s = sums[warp + y][g][lane];
+                o[g].x += s.x; o[g].y += s.y; o[g].z += s.z; o[g].w += s.w;
+            }
+            const float4 s = weights[warp + y];
+            l.x += s.x; l.y += s.y; l.z += s.z; l.w += s.w;
+        }
+    }
+    auto store = [&](int e, float m, float sum, auto value) {
+        const int row = row0 + e;
+        if (row >= rows_all) return;
+        const int j = a.by_heads(row), h = row - j * a.heads;
+        const long long token = (long long)own.x * a.q_len + j;
+        const float inv = sum == 0.f ? 0.f : rcp(sum);
+        T* out = (T*)a.out + token * a.out_token + h * a.out_head + 128 * g0 + 32 * w + lane;
+#pragma unroll
+        for (int g = 0; g < GN; ++g) out[128 * g] = from_float<T>(value(o[g]) * inv);
+        if (w == 0 && g0 == 0 && lane == 0 && a.lse) a.lse[token * a.heads + h] = lse_of(m, sum);
+    };
+    store(0, m0, l.x, [](const float4& f) { return f.x; });
+    store(1, m1, l.y, [](const float4& f) { return f.y; });
+    store(2, m2, l.z, [](const float4& f) { return f.z; });
+    store(3, m3, l.w, [](const float4& f) { return f.w; });
 }
 
 namespace {
@@ -943,8 +936,8 @@ FastDiv fast_div(unsigned d, int bits) {
     return FastDiv{(unsigned)(((1ull << shift) + d - 1) / d), (unsigned)shift};
 }
 
-constexpr size_t kOwnerBytes = kMaxGrid * sizeof(int4), kMlBytes = 2 * (size_t)kMaxGrid * kTileRows * sizeof(float2);
-constexpr size_t kAttWorkspace = kOwnerBytes + kMlBytes + 2 * (size_t)kMaxGrid * kPartFloats * sizeof(float);
+constexpr size_t kMadeBytes = kMaxGrid * sizeof(int4), kMlBytes = 2 * (size_t)kMaxGrid * kTileRows * sizeof(float2);
+constexpr size_t kAttWorkspace = kMadeBytes + kMlBytes + 2 * (size_t)kMaxGrid * kPartFloats * sizeof(float);
 
 template <typename T>
 int launch_attention(const CUtensorMap& map, const AttentionArgs& a, int grid, cudaStream_t st) {
@@ -955,7 +948,12 @@ int launch_attention(const CUtensorMap& map, const AttentionArgs& a, int grid, c
     }
     const int r = launch_latent(latent_attention_kernel<T>, dim3((unsigned)grid), kAttThreads, kAttSmem, st, map, a);
     if (r) return r;
-    return launch_latent(latent_combine_kernel<T>, dim3((unsigned)(4 * sm_count())), kCombineThreads, 0, st, a, grid);
+    const long long items = (long long)a.batch * a.lanes * a.blocks_per_lane;
+    const int made = a.by_item ? (int)items : grid;
+    const int team = made <= 18 ? 8 : made <= 64 ? 4 : 1, halves = made <= 4 ? 2 : 1;
+    const dim3 blocks((unsigned)(a.block_rows * team * halves / kCombineWarps), (unsigned)made);
+    return halves == 2 ? launch_latent(latent_combine_kernel<T, 2>, blocks, kCombineThreads, 0, st, a, team)
+                       : launch_latent(latent_combine_kernel<T, 4>, blocks, kCombineThreads, 0, st, a, team);
 }
 
 }  // namespace
@@ -1004,16 +1002,21 @@ extern "C" int vib3_launch_latent_attention_paged(const void* q, long long q_tok
     a.out = out; a.out_token = out_token_stride; a.out_head = out_head_stride;
     a.lse = lse_or_null; a.status = status;
     unsigned char* ws = static_cast<unsigned char*>(workspace);
-    a.owner = reinterpret_cast<int4*>(ws);
-    a.part_ml = reinterpret_cast<float2*>(ws + kOwnerBytes);
-    a.part_o = reinterpret_cast<float4*>(ws + kOwnerBytes + kMlBytes);
-    const int blocks = (int)(((long long)q_len * heads + kTileRows - 1) / kTileRows);
+    a.made_of = reinterpret_cast<int4*>(ws);
+    a.part_ml = reinterpret_cast<float2*>(ws + kMadeBytes);
+    a.part_o = reinterpret_cast<float4*>(ws + kMadeBytes + kMlBytes);
     const int sms = sm_count() < kMaxGrid ? sm_count() : kMaxGrid;
+    const long long rows = (long long)q_len * heads, most_tiles = ((long long)max_pages_per_seq * page_size + kTileKeys - 1) / kTileKeys;
+    // Half row blocks where the whole ones would leave half of the SMs without work: the cache is then read twice (from L2), the
+    // results of a CTA, 128 KB at 30 bytes per cycle, are halved.
+    a.block_rows = rows > 32 && (rows + kTileRows - 1) / kTileRows * batch * most_tiles <= sms ? kTileRows / 2 : kTileRows;
+    const int blocks = (int)((rows + a.block_rows - 1) / a.block_rows);
     a.lanes = blocks <= 8 ? blocks : 1;
     a.blocks_per_lane = blocks / a.lanes;
-    // the kernel counts tiles in 32 bits
-    if ((long long)batch * a.blocks_per_lane * (((long long)max_pages_per_seq * page_size + kTileKeys - 1) / kTileKeys) > 0x7fffffff) return VIB3_ERR_COUNT;
-    a.min_tiles = 2;
+    // the kernel counts tiles (and what a row block costs beside them) in 32 bits
+    if ((long long)batch * a.blocks_per_lane * (most_tiles + kPieceCost) > 0x7fffffff) return VIB3_ERR_COUNT;
+    a.by_item = (long long)batch * blocks <= kMaxGrid;
+    a.min_cost = kMinCost;
     const int grid = sms / a.lanes * a.lanes;
 
     CUtensorMap map;

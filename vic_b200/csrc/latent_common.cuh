@@ -57,9 +57,11 @@ __device__ __forceinline__ void rope_angle(int position, double inv_freq, float 
 // Every latent kernel starts with pdl_enter(): nothing of its inputs is read before the predecessor in the stream has
 // finished (its weights may be what the predecessor wrote), and the successor may start only after that, so that a launch
 // that reads older data before its own wait still finds it complete.  What overlaps is the launch itself.
+__device__ __forceinline__ void pdl_wait_only() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_enter() {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    pdl_wait_only();
+    pdl_release();
 }
 
 template <class K, class... Args>
