@@ -18,16 +18,11 @@
 // Per tile the pipe is busy 36 x 32 + 16 x 48 = 1920 cycles, HBM's share of an SM 3150.  What decides is how long a tile stays in
 // shared memory: load 2800 to 3500, S 1150, softmax 700, O 900 cycles.  With all of Q in shared memory there is room for two tiles
 // and a tile took 3500 cycles; with six of its nine chunks in tensor memory for two and three quarters.
-#include <cuda.h>
-
-#include "latent_common.cuh"
+#include "latent_tc.cuh"
 
 namespace vib3 {
 
-int sm_count();
-
 constexpr int kTileKeys = 64, kTileRows = 64;
-constexpr int kChunkBytes = 64 * 128;                     // 64 rows of 64 values, 128-byte swizzle
 constexpr int kChunks = kLatentRow / 64;                  // 9: eight of the latent, one of position values
 constexpr int kTileBytes = kChunks * kChunkBytes;
 // Shared memory: the part of Q that tensor memory has no room for, a ring of latent chunk pairs, places for position values (then P).
@@ -134,6 +129,9 @@ struct Walk {
     }
 };
 
+template <typename T> constexpr uint32_t kIdescS = idesc<T>(64, 64, false, false);
+template <typename T> constexpr uint32_t kIdescO = idesc<T>(128, 64, true, false);
+
 struct AttShared {
     uint64_t kv_full[kTiles], slot_empty[kSlots], rope_empty[kTiles];
     uint64_t s_full, s_free, p_full[2], pv_done[2], q_full, drain[2];
@@ -146,68 +144,6 @@ struct AttShared {
 static_assert(kMiscOff + sizeof(AttShared) <= 227 * 1024, "shared memory of a CTA");
 constexpr int kAttSmem = kMiscOff + (int)sizeof(AttShared);
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void bar_init(uint64_t* bar, unsigned count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint64_t* bar, unsigned bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-// Waits for the phase with this parity; gives up, with false, after about four seconds (a try comes back after some 4 us).
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, unsigned parity) {
-    const uint32_t addr = smem_u32(bar);
-    uint32_t ok = 0;
-    for (unsigned it = 0; !ok && it < (1u << 20); ++it)
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
-    return ok != 0;
-}
-// The same for a whole warp, whose lanes have to agree (they meet again in warp-wide instructions).
-__device__ __forceinline__ bool bar_wait_warp(uint64_t* bar, unsigned parity) { return __all_sync(0xffffffffu, bar_wait(bar, parity)); }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-// One lane of the warp, the same one every time: behind elect.sync MMAs and tensor copies issue back to back.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t p;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
-    return p != 0;
-}
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-// Shared-memory operands with 128-byte swizzle.  K-major: rows of 128 bytes, eight of them 1024 bytes.  MN-major: 64 values
-// contiguous per key, eight keys 1024 bytes, the next 64 values a chunk further.
-constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | (1u << 16); }
-__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | ((uint32_t)(kChunkBytes >> 4) << 16); }
-// A value that is the same in all lanes, told to the compiler: an MMA takes its operands from uniform registers, and with
-// operands that it had to move there one by one an MMA of this kernel cost 85 cycles instead of the pipe's 32 or 48.
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
-// Operands by the low words of their descriptors (the address); the high words are constants.
-__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
-                 ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kDescHigh) : "memory");
-}
-// The same with the first operand in tensor memory.
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kDescHigh) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -249,9 +185,6 @@ __device__ __forceinline__ bool softmax_any(bool v) {
     return r != 0;
 }
 
-template <typename T> constexpr uint32_t kFormat = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-template <typename T> constexpr uint32_t kIdescS = (1u << 4) | (kFormat<T> << 7) | (kFormat<T> << 10) | (64u / 8 << 17) | (64u / 16 << 24);
-template <typename T> constexpr uint32_t kIdescO = (1u << 4) | (kFormat<T> << 7) | (kFormat<T> << 10) | (1u << 15) | (64u / 8 << 17) | (128u / 16 << 24);
 
 // 16 lanes x 32 columns: thread t has columns 8 x + 2 (t & 3) + {0, 1} of lane t / 4 (registers 4 x, 4 x + 1) and of lane t / 4 + 8.
 __device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t* r) {
@@ -259,13 +192,6 @@ __device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t* r) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr) : "memory");
 }
-// 32 lanes x 32 columns, a lane per thread.
-__device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t* r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                 : "r"(taddr) : "memory");
-}
-
 __device__ __forceinline__ void tmem_st_16x32(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
@@ -913,22 +839,6 @@ __global__ void __launch_bounds__(kCombineThreads, 2) latent_combine_kernel(cons
 
 namespace {
 
-typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn tensor_map_encoder() {
-    static EncodeFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult r;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess) {
-            p = nullptr;
-            (void)cudaGetLastError();
-        }
-        return reinterpret_cast<EncodeFn>(p);
-    }();
-    return fn;
-}
-
 FastDiv fast_div(unsigned d, int bits) {
     int log = 0;
     while ((1u << log) < d) ++log;
@@ -941,12 +851,9 @@ constexpr size_t kAttWorkspace = kMadeBytes + kMlBytes + 2 * (size_t)kMaxGrid * 
 
 template <typename T>
 int launch_attention(const CUtensorMap& map, const AttentionArgs& a, int grid, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(latent_attention_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttSmem);
-    if (e != cudaSuccess) {
-        (void)cudaGetLastError();
-        return (int)e;
-    }
-    const int r = launch_latent(latent_attention_kernel<T>, dim3((unsigned)grid), kAttThreads, kAttSmem, st, map, a);
+    int r = allow_smem<latent_attention_kernel<T>>(kAttSmem);
+    if (r) return r;
+    r = launch_latent(latent_attention_kernel<T>, dim3((unsigned)grid), kAttThreads, kAttSmem, st, map, a);
     if (r) return r;
     const long long items = (long long)a.batch * a.lanes * a.blocks_per_lane;
     const int made = a.by_item ? (int)items : grid;
@@ -987,8 +894,7 @@ extern "C" int vib3_launch_latent_attention_paged(const void* q, long long q_tok
         return VIB3_ERR_ALIGN;
     if (workspace_bytes < kAttWorkspace) return VIB3_ERR_CAPACITY;
     if (batch == 0 || q_len == 0) return VIB3_OK;
-    const EncodeFn encode = tensor_map_encoder();
-    if (!encode) return VIB3_ERR_UNSUPPORTED;
+    if (!tensor_map_encoder()) return VIB3_ERR_UNSUPPORTED;
 
     AttentionArgs a;
     a.q = q; a.q_token = q_token_stride; a.q_head = q_head_stride;
@@ -1020,12 +926,7 @@ extern "C" int vib3_launch_latent_attention_paged(const void* q, long long q_tok
     const int grid = sms / a.lanes * a.lanes;
 
     CUtensorMap map;
-    const cuuint64_t dims[3] = {(cuuint64_t)kLatentRow, (cuuint64_t)page_size, (cuuint64_t)num_pages};
-    const cuuint64_t strides[2] = {(cuuint64_t)row_stride * 2, (cuuint64_t)page_stride * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)a.box_rows, 1}, one[3] = {1, 1, 1};
-    if (encode(&map, dtype == L_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(cache), dims, strides,
-               box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    if (!map_3d(&map, dtype, cache, kLatentRow, page_size, num_pages, row_stride, page_stride, a.box_rows, 1))
         return VIB3_ERR_SHAPE;
     return dtype == L_F16 ? launch_attention<__half>(map, a, grid, (cudaStream_t)stream)
                           : launch_attention<__nv_bfloat16>(map, a, grid, (cudaStream_t)stream);

@@ -43,6 +43,11 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, f
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v) {
+    const T* t = reinterpret_cast<const T*>(&v);
+    return make_float2(as_float(t[0]), as_float(t[1]));
+}
+
 // Cosine and sine of position * inv_freq.  The angle of a far position has no 32-bit form that keeps its fraction of a turn
 // (at 200,000 the spacing of fp32 is 1/64): it is formed and reduced to [-pi, pi] in 64 bits and only then rounded.
 __device__ __forceinline__ void rope_angle(int position, double inv_freq, float scale, float& c, float& s) {

@@ -4,7 +4,7 @@
 //   vib3_launch_latent_value          per head o . W_uv^T
 // The reference has a scalar kernel for each (vib3_mla_kv_cache_append_kernel, vib3_mla_q_absorb_rope_kernel,
 // vib3_mla_v_reconstruct, cuda/src/kernels.cu:1709, :1679, :1624), for one token and a flat cache.
-#include "latent_common.cuh"
+#include "latent_tc.cuh"
 
 namespace vib3 {
 
@@ -97,153 +97,19 @@ __global__ void __launch_bounds__(kAppendWarps * 32) latent_append_kernel(Append
 }
 
 // ── per-head products ────────────────────────────────────────────────────────────────────────
-// C[t, n] = sum_k A[t, k] B(k, n) for one head, fp32 accumulation on the warp-level tensor instructions.  These products are
-// bound by their bytes, not by their arithmetic: with one token the head matrices are read for two flops per value, with 512 a
-// query's result rows are most of the traffic.
-constexpr int kChunkK = 64;   // columns of K per pipeline stage: 128-byte rows
+// C[t, n] = sum_k A[t, k] B(k, n) for one head.  A CTA takes 128 tokens (fewer are padded with zeros that TMA writes) and n_cols
+// columns; A and B come as chunks of 64 values of K through a ring, the sum stays in tensor memory, and the rounded tile leaves
+// through shared memory as one tensor copy, which leaves out what lies beyond the last token or column.
+//   query: A = q_nope [tokens][nope], B = W_uk[h] [nope][512]: columns contiguous (MN-major)
+//   value: A = o [tokens][512],       B = W_uv[h] [value][512]: K contiguous
+// These products are bound by their bytes: with one token the head matrices are read for two flops per value, with 512 a query's
+// result rows are most of the traffic (and the tensor pipe is busy for a fifth of the time).  So what counts is many bytes in flight
+// with few instructions; warp-level MMAs fed by 16-byte copies spent their time on addresses (500 queries: 32 us).
+constexpr int kHeadTokens = 128, kHeadAChunk = kHeadTokens * 128, kHeadMaxStages = 8;
+constexpr int kHeadThreads = 192;          // copies, MMAs, four warps for the results
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// 16 bytes global -> shared, zeros where !valid (the address is then not read)
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-__device__ __forceinline__ void ldm4(uint32_t a, uint32_t* r) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void ldm2(uint32_t a, uint32_t* r) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void ldm4t(uint32_t a, uint32_t* r) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-template <typename T>
-__device__ __forceinline__ void mma16(float* d, const uint32_t* a, const uint32_t* b) {
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
-}
-
-// One BM x BN tile.  NK: B is stored [n][k] (k contiguous), else [k][n].  Tiles lie in shared memory as rows of 128 bytes (B as
-// [k][n]: 2 BN bytes) whose 16-byte pieces are permuted by the row number, so that the eight rows of a matrix fragment come
-// from different banks.  Rows and columns outside the matrix are zeros, so their values in memory do not matter.
-template <typename T, bool NK, int BM_, int BN_, int WARPS_M, int WARPS_N, int STAGES>
-struct HeadTile {
-    static constexpr int BM = BM_, BN = BN_;
-    static constexpr int kThreads = WARPS_M * WARPS_N * 32;
-    static constexpr int WM = BM / WARPS_M, WN = BN / WARPS_N, MF = WM / 16, NF = WN / 8;
-    static constexpr int kABytes = BM * kChunkK * 2, kBBytes = BN * kChunkK * 2;
-    static constexpr int kOutStride = BN + 8;
-    static constexpr size_t kPipe = (size_t)STAGES * (kABytes + kBBytes), kOut = (size_t)BM * kOutStride * 2;
-    static constexpr size_t kSmem = kPipe > kOut ? kPipe : kOut;
-    static_assert(MF >= 1 && (NF == 1 || NF % 2 == 0) && (NK || NF % 2 == 0), "fragments");
-    static_assert(NK || BN >= 64, "a row of B holds the eight permuted pieces");
-
-    // A: rows t0.. of T rows, a_stride elements apart; B: n0.. of N; the result goes to c (row stride c_stride).
-    static __device__ void run(unsigned char* smem, const T* A, long long a_stride, int t0, int n_tokens, const T* B, int b_stride, int n0,
-                               int N, int K, T* C, long long c_stride) {
-        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-        const int wm = warp / WARPS_N, wn = warp % WARPS_N;
-        const uint32_t base = smem_addr(smem);
-        const int nk = (K + kChunkK - 1) / kChunkK;
-        auto load = [&](int kc) {
-            const uint32_t sa = base + (kc % STAGES) * (kABytes + kBBytes), sb = sa + kABytes;
-            const int k0 = kc * kChunkK;
-#pragma unroll
-            for (int i = tid; i < BM * 8; i += kThreads) {
-                const int r = i >> 3, c = i & 7;
-                const bool ok = t0 + r < n_tokens && k0 + c * 8 < K;
-                cp16(sa + r * 128 + ((c ^ (r & 7)) << 4), ok ? A + (long long)(t0 + r) * a_stride + k0 + c * 8 : A, ok);
-            }
-            if constexpr (NK) {
-#pragma unroll
-                for (int i = tid; i < BN * 8; i += kThreads) {
-                    const int r = i >> 3, c = i & 7;
-                    const bool ok = n0 + r < N && k0 + c * 8 < K;
-                    cp16(sb + r * 128 + ((c ^ (r & 7)) << 4), ok ? B + (long long)(n0 + r) * b_stride + k0 + c * 8 : B, ok);
-                }
-            } else {
-                constexpr int P = BN / 8;   // 16-byte pieces of a row
-#pragma unroll
-                for (int i = tid; i < kChunkK * P; i += kThreads) {
-                    const int r = i / P, c = i % P;
-                    const bool ok = k0 + r < K && n0 + c * 8 < N;
-                    cp16(sb + r * (BN * 2) + ((c ^ (r & 7)) << 4), ok ? B + (long long)(k0 + r) * b_stride + n0 + c * 8 : B, ok);
-                }
-            }
-        };
-        float acc[MF][NF][4];
-#pragma unroll
-        for (int i = 0; i < MF; ++i)
-#pragma unroll
-            for (int j = 0; j < NF; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
-#pragma unroll
-        for (int s = 0; s < STAGES; ++s) {
-            if (s < nk) load(s);
-            cp_commit();
-        }
-        for (int kc = 0; kc < nk; ++kc) {
-            cp_wait<STAGES - 1>();
-            __syncthreads();
-            const uint32_t sa = base + (kc % STAGES) * (kABytes + kBBytes), sb = sa + kABytes;
-#pragma unroll
-            for (int ks = 0; ks < kChunkK / 16; ++ks) {
-                uint32_t af[MF][4], bf[NF][2];
-#pragma unroll
-                for (int i = 0; i < MF; ++i) {
-                    const int r = wm * WM + i * 16 + (lane & 15), c = ks * 2 + (lane >> 4);
-                    ldm4(sa + r * 128 + ((c ^ (r & 7)) << 4), af[i]);
-                }
-                if constexpr (NF == 1) {
-                    const int r = wn * WN + (lane & 7), c = ks * 2 + ((lane >> 3) & 1);
-                    ldm2(sb + r * 128 + ((c ^ (r & 7)) << 4), bf[0]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < NF; j += 2) {
-                        if constexpr (NK) {
-                            const int r = wn * WN + j * 8 + (lane & 7) + ((lane >> 4) << 3), c = ks * 2 + ((lane >> 3) & 1);
-                            ldm4(sb + r * 128 + ((c ^ (r & 7)) << 4), bf[j]);
-                        } else {
-                            const int r = ks * 16 + (lane & 15), c = (wn * WN + j * 8) / 8 + (lane >> 4);
-                            ldm4t(sb + r * (BN * 2) + ((c ^ (r & 7)) << 4), bf[j]);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < MF; ++i)
-#pragma unroll
-                    for (int j = 0; j < NF; ++j) mma16<T>(acc[i][j], af[i], bf[j]);
-            }
-            __syncthreads();
-            if (kc + STAGES < nk) load(kc + STAGES);
-            cp_commit();
-        }
-        // the tile through shared memory, so that a row leaves in 16-byte pieces
-        cp_wait<0>();
-        __syncthreads();
-        T* so = reinterpret_cast<T*>(smem);
-#pragma unroll
-        for (int i = 0; i < MF; ++i)
-#pragma unroll
-            for (int j = 0; j < NF; ++j) {
-                const int r = wm * WM + i * 16 + (lane >> 2), c = wn * WN + j * 8 + (lane & 3) * 2;
-                *reinterpret_cast<uint32_t*>(so + r * kOutStride + c) = pack2<T>(acc[i][j][0], acc[i][j][1]);
-                *reinterpret_cast<uint32_t*>(so + (r + 8) * kOutStride + c) = pack2<T>(acc[i][j][2], acc[i][j][3]);
-            }
-        __syncthreads();
-        for (int i = tid; i < BM * (BN / 8); i += kThreads) {
-            const int r = i / (BN / 8), c = (i % (BN / 8)) * 8;
-            if (t0 + r < n_tokens && n0 + c < N)
-                *reinterpret_cast<uint4*>(C + (long long)(t0 + r) * c_stride + n0 + c) = *reinterpret_cast<const uint4*>(so + r * kOutStride + c);
-        }
-    }
+struct HeadMaps {
+    CUtensorMap a, b, c;
 };
 
 struct HeadArgs {
@@ -259,93 +125,196 @@ struct HeadArgs {
     const double* inv_freq;
     float rope_scale;
     int pairs;
-    int product_blocks;          // blocks of the product; the others rotate
+    // the split
+    int k_steps, n_cols, col_blocks, stages, product_blocks;   // MMAs of 16 along K, columns of a CTA, ...; the other blocks rotate
 };
 
-// blockIdx.x = (tile of tokens * heads + head) * column blocks + column block.
-template <typename T, class Tile>
-__global__ void __launch_bounds__(Tile::kThreads) latent_value_kernel(HeadArgs g) {
-    extern __shared__ __align__(128) unsigned char smem[];
-    pdl_enter();
-    const int nb = (g.dim + Tile::BN - 1) / Tile::BN;
-    const int n = blockIdx.x % nb, h = blockIdx.x / nb % g.heads, tt = blockIdx.x / nb / g.heads;
-    Tile::run(smem, (const T*)g.a + h * g.a_head, g.a_token, tt * Tile::BM, g.n_tokens, (const T*)g.w + h * g.w_head, kRank, n * Tile::BN,
-              g.dim, kRank, (T*)g.out + h * g.out_head, g.out_token);
-}
+constexpr int kRotateHeads = 8;    // heads that share one evaluation of a token's angles
 
-constexpr int kRotateHeads = 16;   // heads that share one evaluation of a token's angles
-
-template <typename T, class Tile>
-__global__ void __launch_bounds__(Tile::kThreads) latent_query_kernel(HeadArgs g) {
-    extern __shared__ __align__(128) unsigned char smem[];
-    pdl_enter();
-    if ((int)blockIdx.x < g.product_blocks) {
-        constexpr int nb = kRank / Tile::BN;
-        const int n = blockIdx.x % nb, h = blockIdx.x / nb % g.heads, tt = blockIdx.x / nb / g.heads;
-        Tile::run(smem, (const T*)g.a + h * g.a_head, g.a_token, tt * Tile::BM, g.n_tokens, (const T*)g.w + h * g.w_head, kRank,
-                  n * Tile::BN, kRank, g.dim, (T*)g.out + h * g.out_head, g.out_token);
-        return;
-    }
-    // the rotation: a warp turns the 64 position values of up to 16 heads of one token
-    const int lane = threadIdx.x & 31;
-    const int groups = (g.heads + kRotateHeads - 1) / kRotateHeads;
-    const int item = (blockIdx.x - g.product_blocks) * (Tile::kThreads / 32) + (threadIdx.x >> 5);
+// The 64 position values of up to eight heads of a token, by half a warp: a lane turns two pairs.
+template <typename T>
+__device__ __forceinline__ void rotate_heads(const HeadArgs& g) {
+    const int groups = (g.heads + kRotateHeads - 1) / kRotateHeads, l = threadIdx.x & 15;
+    const int item = (blockIdx.x - g.product_blocks) * (kHeadThreads / 16) + (threadIdx.x >> 4);
     if (item >= g.n_tokens * groups) return;
     const int t = item / groups, h0 = item % groups * kRotateHeads, hn = min(kRotateHeads, g.heads - h0);
     const T* q = (const T*)g.a + t * g.a_token + h0 * g.a_head + g.dim;
     T* o = (T*)g.out + t * g.out_token + h0 * g.out_head + kRank;
-    const int i0 = g.pairs ? 2 * lane : lane, i1 = g.pairs ? 2 * lane + 1 : lane + 32;
-    float c, s;
-    rope_angle(g.positions[t], g.inv_freq[lane], g.rope_scale, c, s);
-#pragma unroll 8
-    for (int h = 0; h < hn; ++h) {
-        const T* x = q + h * g.a_head;
-        T* y = o + h * g.out_head;
-        const float a = as_float(x[i0]), b = as_float(x[i1]);
-        y[i0] = from_float<T>(a * c - b * s);
-        y[i1] = from_float<T>(b * c + a * s);
+    // neighbours: values 4 l .. 4 l + 3; halves: 2 l, 2 l + 1 and the same 32 further
+    const int x = g.pairs ? 4 * l : 2 * l, y = g.pairs ? 4 * l + 2 : 2 * l + 32;
+    uint32_t u[kRotateHeads], v[kRotateHeads];
+#pragma unroll
+    for (int h = 0; h < kRotateHeads; ++h)
+        if (h < hn) {
+            u[h] = *reinterpret_cast<const uint32_t*>(q + h * g.a_head + x);
+            v[h] = *reinterpret_cast<const uint32_t*>(q + h * g.a_head + y);
+        }
+    float c0, s0, c1, s1;
+    rope_angle(g.positions[t], g.inv_freq[2 * l], g.rope_scale, c0, s0);
+    rope_angle(g.positions[t], g.inv_freq[2 * l + 1], g.rope_scale, c1, s1);
+#pragma unroll
+    for (int h = 0; h < kRotateHeads; ++h)
+        if (h < hn) {
+            const float2 p = unpack2<T>(u[h]), r = unpack2<T>(v[h]);
+            uint32_t a, b;
+            if (g.pairs) {
+                a = pack2<T>(p.x * c0 - p.y * s0, p.y * c0 + p.x * s0);
+                b = pack2<T>(r.x * c1 - r.y * s1, r.y * c1 + r.x * s1);
+            } else {
+                a = pack2<T>(p.x * c0 - r.x * s0, p.y * c1 - r.y * s1);
+                b = pack2<T>(r.x * c0 + p.x * s0, r.y * c1 + p.y * s1);
+            }
+            *reinterpret_cast<uint32_t*>(o + h * g.out_head + x) = a;
+            *reinterpret_cast<uint32_t*>(o + h * g.out_head + y) = b;
+        }
+}
+
+// blockIdx.x = (tile of tokens * heads + head) * column blocks + column block, then the rotating blocks.
+template <typename T, bool QUERY>
+__global__ void __launch_bounds__(kHeadThreads) latent_head_kernel(const __grid_constant__ HeadMaps maps, const HeadArgs g) {
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ uint64_t full[kHeadMaxStages], empty[kHeadMaxStages], done;
+    __shared__ uint32_t tmem_at;
+    if (QUERY && (int)blockIdx.x >= g.product_blocks) {
+        pdl_enter();
+        rotate_heads<T>(g);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    // (the swizzle goes by the address, and a static array stands before the dynamic memory)
+    const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
+    const uint32_t a_bytes = kHeadAChunk, b_bytes = (uint32_t)g.n_cols * 128, stage_bytes = a_bytes + b_bytes;
+    const int chunks = (g.k_steps + 3) >> 2;
+    const uint32_t tmem_cols = (uint32_t)g.n_cols;      // 64, 128 or 256
+    if (tid == 0) {
+        for (int s = 0; s < g.stages; ++s) {
+            bar_init(&full[s], 1);
+            bar_init(&empty[s], 1);
+        }
+        bar_init(&done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_at)), "r"(tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = uniform(tmem_at);
+    pdl_enter();
+    const int col = blockIdx.x % g.col_blocks * g.n_cols, h = blockIdx.x / g.col_blocks % g.heads, t0 = blockIdx.x / g.col_blocks / g.heads * kHeadTokens;
+    bool ok = true;
+    if (warp == 0) {
+        if (elect_one()) {
+            for (int c = 0; c < chunks; ++c) {
+                const int s = c % g.stages;
+                if (c >= g.stages && !bar_wait(&empty[s], (c / g.stages - 1) & 1)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t at = base + s * stage_bytes;
+                bar_expect(&full[s], stage_bytes);
+                tma_load_3d(at, &maps.a, 64 * c, h, t0, &full[s]);
+                if (QUERY)
+                    for (int n = 0; n < g.n_cols / 64; ++n) tma_load_3d(at + a_bytes + n * kChunkBytes, &maps.b, col + 64 * n, 64 * c, h, &full[s]);
+                else
+                    tma_load_3d(at + a_bytes, &maps.b, 64 * c, col, h, &full[s]);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const uint32_t id = uniform(idesc<T>(128, (uint32_t)g.n_cols, false, QUERY));
+        for (int c = 0; c < chunks; ++c) {
+            const int s = c % g.stages, steps = min(4, g.k_steps - 4 * c);
+            ok = ok && bar_wait_warp(&full[s], (c / g.stages) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t at = base + s * stage_bytes, ad = uniform(desc_k(at)), bd = uniform(QUERY ? desc_mn(at + a_bytes) : desc_k(at + a_bytes));
+            if (elect_one()) {
+                for (int k = 0; k < steps; ++k) umma_ss(tmem, ad + k * 2, bd + k * (QUERY ? 2048 / 16 : 2), id, (uint32_t)(c + k > 0));
+                umma_commit(&empty[s]);
+                if (c == chunks - 1) umma_commit(&done);
+            }
+            __syncwarp();
+        }
+        if (!ok) {      // what was issued has to be through before the tensor memory is freed
+            if (elect_one()) umma_commit(&done);
+            __syncwarp();
+        }
+        bar_wait_warp(&done, 0);
+    } else {
+        // The tile to shared memory, in the place of operands that no MMA reads any more: as chunks of 64 columns, the tensor copy's layout.
+        ok = bar_wait_warp(&done, 0);
+        tc_fence_after();
+        const int row = 32 * (warp & 3) + lane;
+        for (int x = 0; x < g.n_cols / 32; ++x) {
+            uint32_t o[32];
+            tmem_ld_32x32(tmem + 32 * x + ((uint32_t)(32 * (warp & 3)) << 16), o);
+            tmem_ld_wait();
+            unsigned char* to = smem + (base - smem_u32(smem)) + (x >> 1) * kHeadAChunk + row * 128;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint4 b;
+                b.x = pack2<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1]));
+                b.y = pack2<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
+                b.z = pack2<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
+                b.w = pack2<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
+                *reinterpret_cast<uint4*>(to + ((((x & 1) * 4 + i) ^ (row & 7)) << 4)) = b;
+            }
+        }
+        proxy_fence();
+        tc_fence_before();
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (warp == 2 && ok && elect_one()) {
+            for (int n = 0; n < g.n_cols / 64; ++n)
+                asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
+                             ::"l"(&maps.c), "r"(col + 64 * n), "r"(h), "r"(t0), "r"(base + n * kHeadAChunk) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
     }
 }
 
 namespace {
 
-template <class K>
-int allow_smem(K kernel, size_t bytes) {
-    if (bytes <= 48 * 1024) return 0;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e != cudaSuccess) (void)cudaGetLastError();
-    return (int)e;
-}
-
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-template <typename T, class Tile>
-int launch_value(const HeadArgs& g, cudaStream_t st) {
-    const int e = allow_smem(latent_value_kernel<T, Tile>, Tile::kSmem);
+template <typename T, bool QUERY>
+int launch_heads(HeadArgs g, int dtype, cudaStream_t st) {
+    if (!tensor_map_encoder()) return VIB3_ERR_UNSUPPORTED;
+    const int tiles = ceil_div(g.n_tokens, kHeadTokens), n_all = QUERY ? kRank : g.dim, k_all = QUERY ? g.dim : kRank;
+    g.k_steps = k_all / 16;
+    // The widest columns that still give every SM a CTA (a wider one reads A less often).
+    g.n_cols = 256;
+    while (g.n_cols > 64 && (g.n_cols >= 2 * n_all || tiles * g.heads * ceil_div(n_all, g.n_cols) < sm_count())) g.n_cols /= 2;
+    g.col_blocks = ceil_div(n_all, g.n_cols);
+    g.product_blocks = tiles * g.heads * g.col_blocks;
+    // All of K in flight at once where 104 KB allow it, so that two CTAs share an SM; at least two stages (a 256-column stage has 48 KB).
+    const int stage = kHeadAChunk + g.n_cols * 128, chunks = ceil_div(k_all, 64);
+    g.stages = chunks < 104 * 1024 / stage ? chunks : 104 * 1024 / stage;
+    if (g.stages > kHeadMaxStages) g.stages = kHeadMaxStages;
+    const int out_bytes = kHeadTokens * g.n_cols * 2, ring = g.stages * stage, smem = 1024 + (ring > out_bytes ? ring : out_bytes);
+    const int e = allow_smem<latent_head_kernel<T, QUERY>>(1024 + 104 * 1024);
     if (e) return e;
-    const dim3 grid((unsigned)(ceil_div(g.dim, Tile::BN) * g.heads * ceil_div(g.n_tokens, Tile::BM)));
-    return launch_latent(latent_value_kernel<T, Tile>, grid, Tile::kThreads, Tile::kSmem, st, g);
-}
-
-template <typename T, class Tile>
-int launch_query(HeadArgs g, cudaStream_t st) {
-    const int e = allow_smem(latent_query_kernel<T, Tile>, Tile::kSmem);
-    if (e) return e;
-    g.product_blocks = kRank / Tile::BN * g.heads * ceil_div(g.n_tokens, Tile::BM);
-    const int rotate = ceil_div(g.n_tokens * ceil_div(g.heads, kRotateHeads), Tile::kThreads / 32);
-    return launch_latent(latent_query_kernel<T, Tile>, dim3((unsigned)(g.product_blocks + rotate)), Tile::kThreads, Tile::kSmem, st, g);
-}
-
-template <typename T>
-int value_of(const HeadArgs& g, cudaStream_t st) {
-    if (g.n_tokens <= 16) return launch_value<T, HeadTile<T, true, 16, 32, 1, 4, 8>>(g, st);
-    return launch_value<T, HeadTile<T, true, 64, 64, 2, 4, 4>>(g, st);
-}
-
-template <typename T>
-int query_of(const HeadArgs& g, cudaStream_t st) {
-    if (g.n_tokens <= 16) return launch_query<T, HeadTile<T, false, 16, 128, 1, 4, 2>>(g, st);
-    return launch_query<T, HeadTile<T, false, 64, 128, 2, 4, 2>>(g, st);
+    HeadMaps maps;
+    const long long width = QUERY ? g.dim + kRope : kRank, out_width = QUERY ? kLatentRow : g.dim;
+    // (a dimension of one has no stride that matters)
+    const long long at = g.n_tokens > 1 ? g.a_token : width, ah = g.heads > 1 ? g.a_head : width, ot = g.n_tokens > 1 ? g.out_token : out_width,
+                    oh = g.heads > 1 ? g.out_head : out_width, wh = g.heads > 1 ? g.w_head : (long long)k_all * n_all;
+    if (!map_3d(&maps.a, dtype, g.a, width, g.heads, g.n_tokens, ah, at, 1, kHeadTokens) ||
+        !(QUERY ? map_3d(&maps.b, dtype, g.w, kRank, g.dim, g.heads, kRank, wh, 64, 1) : map_3d(&maps.b, dtype, g.w, kRank, g.dim, g.heads, kRank, wh, g.n_cols, 1)) ||
+        !map_3d(&maps.c, dtype, g.out, out_width, g.heads, g.n_tokens, oh, ot, 1, kHeadTokens))
+        return VIB3_ERR_SHAPE;
+    const int rotate = QUERY ? ceil_div(g.n_tokens * ceil_div(g.heads, kRotateHeads), kHeadThreads / 16) : 0;
+    return launch_latent(latent_head_kernel<T, QUERY>, dim3((unsigned)(g.product_blocks + rotate)), kHeadThreads, (size_t)smem, st, maps, g);
 }
 
 bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
@@ -404,21 +373,21 @@ extern "C" int vib3_launch_latent_query(const void* q, long long q_token_stride,
                                         void* out, long long out_token_stride, long long out_head_stride, int n_tokens, int heads, int nope,
                                         int dtype, void* stream) {
     HeadArgs g{q, q_token_stride, q_head_stride, w_uk, w_head_stride, out, out_token_stride, out_head_stride, n_tokens, heads, nope,
-               positions, inv_freq, rope_scale, pairs, 0};
+               positions, inv_freq, rope_scale, pairs};
     if (!positions || !inv_freq) return VIB3_ERR_NULL;
     const int e = check_heads(g, dtype, nope + kRope, kLatentRow);
     if (e) return e;
     if (n_tokens == 0) return VIB3_OK;
-    return dtype == L_F16 ? query_of<__half>(g, (cudaStream_t)stream) : query_of<__nv_bfloat16>(g, (cudaStream_t)stream);
+    return dtype == L_F16 ? launch_heads<__half, true>(g, dtype, (cudaStream_t)stream) : launch_heads<__nv_bfloat16, true>(g, dtype, (cudaStream_t)stream);
 }
 
 extern "C" int vib3_launch_latent_value(const void* o, long long o_token_stride, long long o_head_stride, const void* w_uv,
                                         long long w_head_stride, void* out, long long out_token_stride, long long out_head_stride,
                                         int n_tokens, int heads, int value, int dtype, void* stream) {
     HeadArgs g{o, o_token_stride, o_head_stride, w_uv, w_head_stride, out, out_token_stride, out_head_stride, n_tokens, heads, value,
-               nullptr, nullptr, 1.f, 0, 0};
+               nullptr, nullptr, 1.f, 0};
     const int e = check_heads(g, dtype, kRank, value);
     if (e) return e;
     if (n_tokens == 0) return VIB3_OK;
-    return dtype == L_F16 ? value_of<__half>(g, (cudaStream_t)stream) : value_of<__nv_bfloat16>(g, (cudaStream_t)stream);
+    return dtype == L_F16 ? launch_heads<__half, false>(g, dtype, (cudaStream_t)stream) : launch_heads<__nv_bfloat16, false>(g, dtype, (cudaStream_t)stream);
 }

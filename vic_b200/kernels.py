@@ -311,80 +311,110 @@ def select_local_experts(ids, weights, top_k: int, expert_lo: int, expert_hi: in
 
 
 # ── latent attention ─────────────────────────────────────────────────────────────────────────
+# (One look at a tensor's shape, strides and dtype each: a decode step makes four of these calls per layer, and what a launch takes
+# on the device is less than ten such looks.)
 
 LATENT_RANK, LATENT_ROPE = 512, 64
 LATENT_ROW = LATENT_RANK + LATENT_ROPE
 _X_CODES = {torch.float32: X_F32, torch.float16: X_F16, torch.bfloat16: X_BF16}
+_I32, _I64, _F32, _F64 = torch.int32, torch.int64, torch.float32, torch.float64
 
 
-def _require(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
-def _on_device(*tensors) -> None:
-    """The operands lie on the current device: a launch on another one would read through a foreign context."""
+def _device() -> int:
+    """The current device.  The operands have to lie on it: a launch on another one would read through a foreign context."""
     if not torch.cuda.is_initialized():
         torch.cuda.init()
-    dev = torch._C._cuda_getDevice()
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"operands have to be on the current device (cuda:{dev}), got {t.device}")
+    return torch._C._cuda_getDevice()
+
+
+def _foreign(*tensors) -> ValueError:
+    return ValueError(f"operands have to be on the current device (cuda:{_device()}), got {[str(t.device) for t in tensors if t is not None]}")
 
 
 def latent_append(kv: torch.Tensor, norm_weight: Optional[torch.Tensor], eps: float, positions: torch.Tensor, slots: torch.Tensor,
-                  inv_freq: torch.Tensor, cache: torch.Tensor, pairs: bool = True, rope_scale: float = 1.0, status=None,
-                  stream: Optional[int] = None) -> None:
+                  inv_freq: torch.Tensor, cache: torch.Tensor, pairs: bool = True, rope_scale: float = 1.0,
+                  status: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> None:
     """Rows of latent attention into the paged cache (the reference's MLA cache append, cuda/src/kernels.cu:1709, for T tokens):
     kv [T, 576] fp32 / fp16 / bf16 -> cache [pages, page_size, 576] fp16 / bf16 at ``slots`` [T] int64 (page * page_size + row;
     negative: skipped), the first 512 values RMS-normalised with ``norm_weight`` [512] (the cache's dtype; None: not
     normalised), the other 64 rotated by ``positions`` [T] int32 * ``inv_freq`` [32] float64.  ``pairs``: neighbouring values
     turn together (else values 32 apart).  ``status`` [1] int32 receives VIB3_STATUS_MISSING_PAGE for a slot beyond the cache."""
-    T = positions.shape[0]
-    _require(kv.dim() == 2 and kv.shape == (T, LATENT_ROW) and kv.stride(1) == 1, "kv: [T, 576] with contiguous rows expected")
-    _require(cache.dim() == 3 and cache.shape[2] == LATENT_ROW and cache.stride(2) == 1, "cache: [pages, page_size, 576] with contiguous rows expected")
-    _require(slots.shape == (T,) and slots.dtype == torch.int64 and slots.is_contiguous(), "slots: contiguous int64 [T] expected")
-    _require(positions.dim() == 1 and positions.dtype == torch.int32 and positions.is_contiguous(), "positions: contiguous int32 [T] expected")
-    _require(inv_freq.shape == (LATENT_ROPE // 2,) and inv_freq.dtype == torch.float64 and inv_freq.is_contiguous(), "inv_freq: contiguous float64 [32] expected")
-    _require(kv.dtype in _X_CODES and cache.dtype in (torch.float16, torch.bfloat16), "kv: fp32, fp16 or bf16; cache: fp16 or bf16")
-    _require(norm_weight is None or (norm_weight.shape == (LATENT_RANK,) and norm_weight.dtype == cache.dtype and norm_weight.is_contiguous()),
-             "norm_weight: contiguous [512] of the cache's dtype expected")
-    _on_device(kv, norm_weight, positions, slots, inv_freq, cache, status)
-    check("latent_append", lib().vib3_launch_latent_append_paged(
-        kv.data_ptr(), _X_CODES[kv.dtype], kv.stride(0), _ptr(norm_weight), eps, positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(),
-        rope_scale, int(pairs), T, cache.data_ptr(), _X_CODES[cache.dtype], cache.shape[0], cache.shape[1], cache.stride(0), cache.stride(1),
-        _ptr(status), _stream(stream)))
+    (T, W), (kv_stride, k1) = kv.shape, kv.stride()
+    (pages, page, R), (page_stride, row_stride, c1) = cache.shape, cache.stride()
+    code, dt = _X_CODES.get(kv.dtype), cache.dtype
+    if W != LATENT_ROW or k1 != 1 or code is None:
+        raise ValueError("kv: fp32, fp16 or bf16 [T, 576] with contiguous rows expected")
+    if R != LATENT_ROW or c1 != 1 or (dt != torch.bfloat16 and dt != torch.float16):
+        raise ValueError("cache: fp16 or bf16 [pages, page_size, 576] with contiguous rows expected")
+    if slots.shape != (T,) or slots.dtype != _I64 or not slots.is_contiguous():
+        raise ValueError("slots: contiguous int64 [T] expected")
+    if positions.shape != (T,) or positions.dtype != _I32 or not positions.is_contiguous():
+        raise ValueError("positions: contiguous int32 [T] expected")
+    if inv_freq.shape != (LATENT_ROPE // 2,) or inv_freq.dtype != _F64 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq: contiguous float64 [32] expected")
+    if norm_weight is not None and (norm_weight.shape != (LATENT_RANK,) or norm_weight.dtype != dt or not norm_weight.is_contiguous()):
+        raise ValueError("norm_weight: contiguous [512] of the cache's dtype expected")
+    if not (_device() == kv.get_device() == cache.get_device() == slots.get_device() == positions.get_device() == inv_freq.get_device()
+            == (kv if norm_weight is None else norm_weight).get_device() == (kv if status is None else status).get_device()):
+        raise _foreign(kv, cache, slots, positions, inv_freq, norm_weight, status)
+    err = lib().vib3_launch_latent_append_paged(
+        kv.data_ptr(), code, kv_stride, 0 if norm_weight is None else norm_weight.data_ptr(), eps, positions.data_ptr(), slots.data_ptr(),
+        inv_freq.data_ptr(), rope_scale, 1 if pairs else 0, T, cache.data_ptr(), _X_CODES[dt], pages, page, page_stride, row_stride,
+        0 if status is None else status.data_ptr(), _stream(stream))
+    if err:
+        check("latent_append", err)
 
 
 def latent_query(q: torch.Tensor, w_uk: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, out: torch.Tensor,
                  pairs: bool = True, rope_scale: float = 1.0, stream: Optional[int] = None) -> None:
     """The heads' queries in the latent space (cuda/src/kernels.cu:1679 for T tokens): q [T, H, nope + 64], w_uk [H, nope, 512] ->
     out [T, H, 576] = (q[..., :nope] . w_uk, q[..., nope:] rotated).  One 16-bit dtype; w_uk may be a view of [H, nope + value, 512]."""
-    T, H, nope = q.shape[0], w_uk.shape[0], w_uk.shape[1]
-    _require(q.dim() == 3 and q.shape == (T, H, nope + LATENT_ROPE) and q.stride(2) == 1, "q: [T, H, nope + 64] with contiguous rows expected")
-    _require(w_uk.dim() == 3 and w_uk.shape[2] == LATENT_RANK and w_uk.stride(2) == 1 and w_uk.stride(1) == LATENT_RANK, "w_uk: [H, nope, 512] with contiguous heads expected")
-    _require(out.shape == (T, H, LATENT_ROW) and out.stride(2) == 1, "out: [T, H, 576] with contiguous rows expected")
-    _require(positions.shape == (T,) and positions.dtype == torch.int32 and positions.is_contiguous(), "positions: contiguous int32 [T] expected")
-    _require(inv_freq.shape == (LATENT_ROPE // 2,) and inv_freq.dtype == torch.float64 and inv_freq.is_contiguous(), "inv_freq: contiguous float64 [32] expected")
-    _require(q.dtype in (torch.float16, torch.bfloat16) and w_uk.dtype == q.dtype and out.dtype == q.dtype, "one dtype, fp16 or bf16, expected")
-    _on_device(q, w_uk, positions, inv_freq, out)
-    check("latent_query", lib().vib3_launch_latent_query(
-        q.data_ptr(), q.stride(0), q.stride(1), w_uk.data_ptr(), w_uk.stride(0), positions.data_ptr(), inv_freq.data_ptr(), rope_scale,
-        int(pairs), out.data_ptr(), out.stride(0), out.stride(1), T, H, nope, _X_CODES[q.dtype], _stream(stream)))
+    (T, H, width), (q0, q1, q2) = q.shape, q.stride()
+    (heads, nope, R), (w0, w1, w2) = w_uk.shape, w_uk.stride()
+    o0, o1, o2 = out.stride()
+    dt = q.dtype
+    if width != nope + LATENT_ROPE or heads != H or q2 != 1:
+        raise ValueError("q: [T, H, nope + 64] with contiguous rows expected")
+    if R != LATENT_RANK or w2 != 1 or w1 != LATENT_RANK:
+        raise ValueError("w_uk: [H, nope, 512] with contiguous heads expected")
+    if out.shape != (T, H, LATENT_ROW) or o2 != 1:
+        raise ValueError("out: [T, H, 576] with contiguous rows expected")
+    if positions.shape != (T,) or positions.dtype != _I32 or not positions.is_contiguous():
+        raise ValueError("positions: contiguous int32 [T] expected")
+    if inv_freq.shape != (LATENT_ROPE // 2,) or inv_freq.dtype != _F64 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq: contiguous float64 [32] expected")
+    if (dt != torch.bfloat16 and dt != torch.float16) or w_uk.dtype != dt or out.dtype != dt:
+        raise ValueError("one dtype, fp16 or bf16, expected")
+    if not (_device() == q.get_device() == w_uk.get_device() == positions.get_device() == inv_freq.get_device() == out.get_device()):
+        raise _foreign(q, w_uk, positions, inv_freq, out)
+    err = lib().vib3_launch_latent_query(
+        q.data_ptr(), q0, q1, w_uk.data_ptr(), w0, positions.data_ptr(), inv_freq.data_ptr(), rope_scale, 1 if pairs else 0, out.data_ptr(),
+        o0, o1, T, H, nope, _X_CODES[dt], _stream(stream))
+    if err:
+        check("latent_query", err)
 
 
 def latent_value(o: torch.Tensor, w_uv: torch.Tensor, out: torch.Tensor, stream: Optional[int] = None) -> None:
     """The heads' outputs from their weighted latents (cuda/src/kernels.cu:1624 for T tokens): o [T, H, 512], w_uv [H, value, 512] ->
     out [T, H, value].  One 16-bit dtype."""
-    T, H, value = o.shape[0], w_uv.shape[0], w_uv.shape[1]
-    _require(o.dim() == 3 and o.shape == (T, H, LATENT_RANK) and o.stride(2) == 1, "o: [T, H, 512] with contiguous rows expected")
-    _require(w_uv.dim() == 3 and w_uv.shape[2] == LATENT_RANK and w_uv.stride(2) == 1 and w_uv.stride(1) == LATENT_RANK, "w_uv: [H, value, 512] with contiguous heads expected")
-    _require(out.shape == (T, H, value) and out.stride(2) == 1, "out: [T, H, value] with contiguous rows expected")
-    _require(o.dtype in (torch.float16, torch.bfloat16) and w_uv.dtype == o.dtype and out.dtype == o.dtype, "one dtype, fp16 or bf16, expected")
-    _on_device(o, w_uv, out)
-    check("latent_value", lib().vib3_launch_latent_value(
-        o.data_ptr(), o.stride(0), o.stride(1), w_uv.data_ptr(), w_uv.stride(0), out.data_ptr(), out.stride(0), out.stride(1), T, H, value,
-        _X_CODES[o.dtype], _stream(stream)))
+    (T, H, width), (i0, i1, i2) = o.shape, o.stride()
+    (heads, value, R), (w0, w1, w2) = w_uv.shape, w_uv.stride()
+    o0, o1, o2 = out.stride()
+    dt = o.dtype
+    if width != LATENT_RANK or i2 != 1 or heads != H:
+        raise ValueError("o: [T, H, 512] with contiguous rows expected")
+    if R != LATENT_RANK or w2 != 1 or w1 != LATENT_RANK:
+        raise ValueError("w_uv: [H, value, 512] with contiguous heads expected")
+    if out.shape != (T, H, value) or o2 != 1:
+        raise ValueError("out: [T, H, value] with contiguous rows expected")
+    if (dt != torch.bfloat16 and dt != torch.float16) or w_uv.dtype != dt or out.dtype != dt:
+        raise ValueError("one dtype, fp16 or bf16, expected")
+    if not (_device() == o.get_device() == w_uv.get_device() == out.get_device()):
+        raise _foreign(o, w_uv, out)
+    err = lib().vib3_launch_latent_value(o.data_ptr(), i0, i1, w_uv.data_ptr(), w0, out.data_ptr(), o0, o1, T, H, value, _X_CODES[dt],
+                                         _stream(stream))
+    if err:
+        check("latent_value", err)
 
 
 def latent_attention_workspace_bytes() -> int:
@@ -392,29 +422,44 @@ def latent_attention_workspace_bytes() -> int:
 
 
 def latent_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, scale: float,
-                     out: torch.Tensor, lse: Optional[torch.Tensor] = None, *, workspace: torch.Tensor, status=None,
-                     stream: Optional[int] = None) -> None:
+                     out: torch.Tensor, lse: Optional[torch.Tensor] = None, *, workspace: torch.Tensor,
+                     status: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> None:
     """Attention in the latent space over the paged cache (cuda/src/kernels.cu:1570 for the newest tokens of a batch): q [B * q_len,
     H, 576] (sequence b's q_len tokens together), cache [pages, page_size, 576], page_table [B, max_pages] int32, seq_lens [B] int32
     (keys of each sequence, its new tokens included) -> out [B * q_len, H, 512] and, if given, lse [B * q_len, H] fp32.  Token j of
     a sequence sees the keys up to position seq_lens - q_len + j; a row that sees none is 0 and -inf.  ``workspace``: a uint8
     tensor of latent_attention_workspace_bytes(), not shared by calls that may overlap."""
-    B, H = seq_lens.shape[0], q.shape[1]
-    T = q.shape[0]
+    (T, H, width), (q0, q1, q2) = q.shape, q.stride()
+    (pages, page, R), (c0, c1, c2) = cache.shape, cache.stride()
+    (B, max_pages), (t0, t1) = page_table.shape, page_table.stride()
+    o0, o1, o2 = out.stride()
+    dt = q.dtype
     q_len = T // B if B else 0
-    _require(q.dim() == 3 and q.shape[2] == LATENT_ROW and q.stride(2) == 1 and q_len * B == T, "q: [B * q_len, H, 576] with contiguous rows expected")
-    _require(cache.dim() == 3 and cache.shape[2] == LATENT_ROW and cache.stride(2) == 1, "cache: [pages, page_size, 576] with contiguous rows expected")
-    _require(page_table.dim() == 2 and page_table.shape[0] == B and page_table.dtype == torch.int32 and page_table.stride(1) == 1, "page_table: int32 [B, max_pages] expected")
-    _require(seq_lens.dim() == 1 and seq_lens.dtype == torch.int32 and seq_lens.is_contiguous(), "seq_lens: contiguous int32 [B] expected")
-    _require(out.shape == (T, H, LATENT_RANK) and out.stride(2) == 1, "out: [B * q_len, H, 512] with contiguous rows expected")
-    _require(lse is None or (lse.shape == (T, H) and lse.dtype == torch.float32 and lse.is_contiguous()), "lse: contiguous fp32 [B * q_len, H] expected")
-    _require(q.dtype in (torch.float16, torch.bfloat16) and cache.dtype == q.dtype and out.dtype == q.dtype, "one dtype, fp16 or bf16, expected")
-    _on_device(q, cache, page_table, seq_lens, out, lse, workspace, status)
-    check("latent_attention", lib().vib3_launch_latent_attention_paged(
-        q.data_ptr(), q.stride(0), q.stride(1), cache.data_ptr(), cache.shape[0], cache.shape[1], cache.stride(0), cache.stride(1),
-        page_table.data_ptr(), page_table.stride(0), page_table.shape[1], seq_lens.data_ptr(), B, q_len, H, scale, _X_CODES[q.dtype],
-        out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-        _ptr(status), _stream(stream)))
+    if width != LATENT_ROW or q2 != 1 or q_len * B != T:
+        raise ValueError("q: [B * q_len, H, 576] with contiguous rows expected")
+    if R != LATENT_ROW or c2 != 1:
+        raise ValueError("cache: [pages, page_size, 576] with contiguous rows expected")
+    if page_table.dtype != _I32 or (t1 != 1 and max_pages > 1):
+        raise ValueError("page_table: int32 [B, max_pages] with contiguous rows expected")
+    if seq_lens.shape != (B,) or seq_lens.dtype != _I32 or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens: contiguous int32 [B] expected")
+    if out.shape != (T, H, LATENT_RANK) or o2 != 1:
+        raise ValueError("out: [B * q_len, H, 512] with contiguous rows expected")
+    if lse is not None and (lse.shape != (T, H) or lse.dtype != _F32 or not lse.is_contiguous()):
+        raise ValueError("lse: contiguous fp32 [B * q_len, H] expected")
+    if (dt != torch.bfloat16 and dt != torch.float16) or cache.dtype != dt or out.dtype != dt:
+        raise ValueError("one dtype, fp16 or bf16, expected")
+    if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("workspace: contiguous uint8 expected")
+    if not (_device() == q.get_device() == cache.get_device() == page_table.get_device() == seq_lens.get_device() == out.get_device()
+            == workspace.get_device() == (q if lse is None else lse).get_device() == (q if status is None else status).get_device()):
+        raise _foreign(q, cache, page_table, seq_lens, out, workspace, lse, status)
+    err = lib().vib3_launch_latent_attention_paged(
+        q.data_ptr(), q0, q1, cache.data_ptr(), pages, page, c0, c1, page_table.data_ptr(), t0, max_pages, seq_lens.data_ptr(), B, q_len, H,
+        scale, _X_CODES[dt], out.data_ptr(), o0, o1, 0 if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.numel(),
+        0 if status is None else status.data_ptr(), _stream(stream))
+    if err:
+        check("latent_attention", err)
 
 
 __all__ = [n for n in dir() if not n.startswith("_")] + ["SCORING_SOFTMAX", "SCORING_SIGMOID"]
