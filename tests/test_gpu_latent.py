@@ -386,3 +386,42 @@ def test_attention_with_sequences_of_no_tokens_between_others(cuda_dev, lens, q_
     cache, table, lens = paged(cuda_dev, lens, 64, torch.bfloat16, 21)
     q = torch.randn(lens.numel() * q_len, heads, ROW, generator=gen(cuda_dev, 22), device=cuda_dev).to(torch.bfloat16)
     check_attention(q, cache, table, lens, 0.07)
+
+
+@pytest.mark.parametrize("which", ["tokens", "heads", "weights", "overlapping"])
+def test_products_of_broadcast_and_overlapping_operands(cuda_dev, which):
+    from vic_b200 import kernels
+    T, H, n, dt, g = 5, 3, 128, torch.bfloat16, gen(cuda_dev, 31)
+    q, w = torch.randn(T, H, n + ROPE, generator=g, device=cuda_dev).to(dt), (torch.randn(H, n, RANK, generator=g, device=cuda_dev) * n ** -0.5).to(dt)
+    if which == "tokens":
+        q = q[:1].expand(T, H, n + ROPE)
+    elif which == "heads":
+        q = q[:, :1].expand(T, H, n + ROPE)
+    elif which == "weights":
+        w = w[:1].expand(H, n, RANK)
+    else:
+        q = torch.randn(4096, generator=g, device=cuda_dev).to(dt).as_strided((T, H, n + ROPE), (8, 200, 1))
+    out, f, pos = torch.empty(T, H, ROW, dtype=dt, device=cuda_dev), inv_freq(cuda_dev), torch.arange(T, dtype=torch.int32, device=cuda_dev)
+    kernels.latent_query(q, w, pos, f, out)
+    a, b = q[..., :n].double().transpose(0, 1), w.double()
+    assert_rounded(out[..., :RANK], torch.bmm(a, b).transpose(0, 1), n * 2.0 ** -23 * torch.bmm(a.abs(), b.abs()).transpose(0, 1))
+    assert_rounded(out[..., RANK:], rotate64(q[..., n:], pos, f, True), 16 * 2.0 ** -24 * 2 * q[..., n:].double().abs().amax(-1, keepdim=True))
+
+
+@pytest.mark.parametrize("tokens", [127, 128, 129, 256, 257])
+@pytest.mark.parametrize("heads", [1, 8, 64])
+def test_products_at_the_borders_of_their_tiles(cuda_dev, tokens, heads):
+    """128 tokens a tile, 64 to 256 columns by the number of heads: rows of another tile or head in their place would show."""
+    from vic_b200 import kernels
+    g, dt = gen(cuda_dev, tokens * heads), torch.float16
+    q, w = torch.randn(tokens, heads, 64 + ROPE, generator=g, device=cuda_dev).to(dt), (torch.randn(heads, 64, RANK, generator=g, device=cuda_dev) / 8).to(dt)
+    out, f, pos = torch.full((tokens, heads, ROW), 9.0, dtype=dt, device=cuda_dev), inv_freq(cuda_dev), torch.arange(tokens, dtype=torch.int32, device=cuda_dev)
+    kernels.latent_query(q, w, pos, f, out, pairs=False)
+    a, b = q[..., :64].double().transpose(0, 1), w.double()
+    assert_rounded(out[..., :RANK], torch.bmm(a, b).transpose(0, 1), 64 * 2.0 ** -23 * torch.bmm(a.abs(), b.abs()).transpose(0, 1))
+    assert_rounded(out[..., RANK:], rotate64(q[..., 64:], pos, f, False), 16 * 2.0 ** -24 * 2 * q[..., 64:].double().abs().amax(-1, keepdim=True))
+    o, v = torch.randn(tokens, heads, RANK, generator=g, device=cuda_dev).to(dt), (torch.randn(heads, 144, RANK, generator=g, device=cuda_dev) / 20).to(dt)
+    y = torch.full((tokens, heads, 144), 9.0, dtype=dt, device=cuda_dev)
+    kernels.latent_value(o, v, y)
+    a, b = o.double().transpose(0, 1), v.double().transpose(1, 2)
+    assert_rounded(y, torch.bmm(a, b).transpose(0, 1), RANK * 2.0 ** -23 * torch.bmm(a.abs(), b.abs()).transpose(0, 1))

@@ -97,15 +97,18 @@ __global__ void __launch_bounds__(kAppendWarps * 32) latent_append_kernel(Append
 }
 
 // ── per-head products ────────────────────────────────────────────────────────────────────────
-// C[t, n] = sum_k A[t, k] B(k, n) for one head.  A CTA takes 128 tokens (fewer are padded with zeros that TMA writes) and n_cols
-// columns; A and B come as chunks of 64 values of K through a ring, the sum stays in tensor memory, and the rounded tile leaves
-// through shared memory as one tensor copy, which leaves out what lies beyond the last token or column.
+// C[t, n] = sum_k A[t, k] B(k, n) for one head.  A tile is 128 tokens (fewer are padded) and 128 or 64 columns; A and B come as
+// chunks of 64 values of K through a ring, the sum stays in tensor memory, and the rounded tile leaves through shared memory as tensor
+// copies, which leave out what lies beyond the last token or column.
 //   query: A = q_nope [tokens][nope], B = W_uk[h] [nope][512]: columns contiguous (MN-major)
 //   value: A = o [tokens][512],       B = W_uv[h] [value][512]: K contiguous
 // These products are bound by their bytes: with one token the head matrices are read for two flops per value, with 512 a query's
 // result rows are most of the traffic (and the tensor pipe is busy for a fifth of the time).  So what counts is many bytes in flight
-// with few instructions; warp-level MMAs fed by 16-byte copies spent their time on addresses (500 queries: 32 us).
-constexpr int kHeadTokens = 128, kHeadAChunk = kHeadTokens * 128, kHeadMaxStages = 8;
+// with few instructions (warp-level MMAs fed by 16-byte copies spent their time on addresses: 500 queries of 64 heads in 32 us), and that
+// reads and writes overlap: two CTAs per SM take tile after tile, the ring runs on across them, and of two accumulators one is
+// stored while the other is filled (a CTA per tile, all of them loading and then all of them storing: 16.7 us).
+constexpr int kHeadTokens = 128, kHeadAChunk = kHeadTokens * 128, kHeadMaxStages = 8, kHeadMaxCols = 128;
+constexpr int kHeadOut = kHeadTokens * kHeadMaxCols * 2, kHeadRing = 64 * 1024;
 constexpr int kHeadThreads = 192;          // copies, MMAs, four warps for the results
 
 struct HeadMaps {
@@ -126,18 +129,15 @@ struct HeadArgs {
     float rope_scale;
     int pairs;
     // the split
-    int k_steps, n_cols, col_blocks, stages, product_blocks;   // MMAs of 16 along K, columns of a CTA, ...; the other blocks rotate
+    int k_steps, n_cols, col_blocks, stages, a_rows, tiles;   // MMAs of 16 along K, columns of a tile, ..., tokens that a copy of A brings
 };
 
 constexpr int kRotateHeads = 8;    // heads that share one evaluation of a token's angles
 
 // The 64 position values of up to eight heads of a token, by half a warp: a lane turns two pairs.
 template <typename T>
-__device__ __forceinline__ void rotate_heads(const HeadArgs& g) {
-    const int groups = (g.heads + kRotateHeads - 1) / kRotateHeads, l = threadIdx.x & 15;
-    const int item = (blockIdx.x - g.product_blocks) * (kHeadThreads / 16) + (threadIdx.x >> 4);
-    if (item >= g.n_tokens * groups) return;
-    const int t = item / groups, h0 = item % groups * kRotateHeads, hn = min(kRotateHeads, g.heads - h0);
+__device__ __forceinline__ void rotate_heads(const HeadArgs& g, int t, int h0) {
+    const int l = threadIdx.x & 15, hn = min(kRotateHeads, g.heads - h0);
     const T* q = (const T*)g.a + t * g.a_token + h0 * g.a_head + g.dim;
     T* o = (T*)g.out + t * g.out_token + h0 * g.out_head + kRank;
     // neighbours: values 4 l .. 4 l + 3; halves: 2 l, 2 l + 1 and the same 32 further
@@ -169,29 +169,28 @@ __device__ __forceinline__ void rotate_heads(const HeadArgs& g) {
         }
 }
 
-// blockIdx.x = (tile of tokens * heads + head) * column blocks + column block, then the rotating blocks.
+// Tile = (tile of tokens * heads + head) * column blocks + column block.
 template <typename T, bool QUERY>
 __global__ void __launch_bounds__(kHeadThreads) latent_head_kernel(const __grid_constant__ HeadMaps maps, const HeadArgs g) {
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ uint64_t full[kHeadMaxStages], empty[kHeadMaxStages], done;
+    __shared__ uint64_t full[kHeadMaxStages], empty[kHeadMaxStages], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_at;
-    if (QUERY && (int)blockIdx.x >= g.product_blocks) {
-        pdl_enter();
-        rotate_heads<T>(g);
-        return;
-    }
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    // (the swizzle goes by the address, and a static array stands before the dynamic memory)
-    const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
-    const uint32_t a_bytes = kHeadAChunk, b_bytes = (uint32_t)g.n_cols * 128, stage_bytes = a_bytes + b_bytes;
+    // (the swizzle goes by the address, and the static arrays stand before the dynamic memory)
+    const uint32_t out_at = (smem_u32(smem) + 1023u) & ~1023u, base = out_at + kHeadOut;
+    // (A's rows behind the copied ones are whatever lies there: the MMA reads them, and their sums are not stored)
+    const uint32_t a_bytes = (uint32_t)g.a_rows * 128, b_bytes = (uint32_t)g.n_cols * 128, stage_bytes = a_bytes + b_bytes;
     const int chunks = (g.k_steps + 3) >> 2;
-    const uint32_t tmem_cols = (uint32_t)g.n_cols;      // 64, 128 or 256
+    const uint32_t tmem_cols = 2 * (uint32_t)g.n_cols;      // 128 or 256
     if (tid == 0) {
         for (int s = 0; s < g.stages; ++s) {
             bar_init(&full[s], 1);
             bar_init(&empty[s], 1);
         }
-        bar_init(&done, 1);
+        for (int s = 0; s < 2; ++s) {
+            bar_init(&acc_full[s], 1);
+            bar_init(&acc_empty[s], 128);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -203,76 +202,124 @@ __global__ void __launch_bounds__(kHeadThreads) latent_head_kernel(const __grid_
     tc_fence_after();
     const uint32_t tmem = uniform(tmem_at);
     pdl_enter();
-    const int col = blockIdx.x % g.col_blocks * g.n_cols, h = blockIdx.x / g.col_blocks % g.heads, t0 = blockIdx.x / g.col_blocks / g.heads * kHeadTokens;
     bool ok = true;
+    int s = 0;              // ring stage and the parity of its use
+    unsigned parity = 0;
+    auto advance = [&] {
+        if (++s == g.stages) {
+            s = 0;
+            parity ^= 1;
+        }
+    };
     if (warp == 0) {
         if (elect_one()) {
-            for (int c = 0; c < chunks; ++c) {
-                const int s = c % g.stages;
-                if (c >= g.stages && !bar_wait(&empty[s], (c / g.stages - 1) & 1)) {
-                    ok = false;
-                    break;
+            int n = 0;      // chunks so far
+            for (int tile = blockIdx.x; ok && tile < g.tiles; tile += gridDim.x) {
+                const int col = tile % g.col_blocks * g.n_cols, h = tile / g.col_blocks % g.heads, t0 = tile / g.col_blocks / g.heads * kHeadTokens;
+                for (int c = 0; c < chunks; ++c, ++n) {
+                    if (n >= g.stages && !bar_wait(&empty[s], parity ^ 1)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t at = base + s * stage_bytes;
+                    bar_expect(&full[s], stage_bytes);
+                    tma_load_3d(at, &maps.a, 64 * c, h, t0, &full[s]);
+                    if (QUERY)
+                        for (int x = 0; x < g.n_cols / 64; ++x) tma_load_3d(at + a_bytes + x * kChunkBytes, &maps.b, col + 64 * x, 64 * c, h, &full[s]);
+                    else
+                        tma_load_3d(at + a_bytes, &maps.b, 64 * c, col, h, &full[s]);
+                    advance();
                 }
-                const uint32_t at = base + s * stage_bytes;
-                bar_expect(&full[s], stage_bytes);
-                tma_load_3d(at, &maps.a, 64 * c, h, t0, &full[s]);
-                if (QUERY)
-                    for (int n = 0; n < g.n_cols / 64; ++n) tma_load_3d(at + a_bytes + n * kChunkBytes, &maps.b, col + 64 * n, 64 * c, h, &full[s]);
-                else
-                    tma_load_3d(at + a_bytes, &maps.b, 64 * c, col, h, &full[s]);
+            }
+            // nothing is in flight to this CTA's memory when it leaves, neither copies nor the releases of their stages
+            for (int x = n > g.stages ? n - g.stages : 0; x < n; ++x) {
+                bar_wait(&full[x % g.stages], (x / g.stages) & 1);
+                if (ok) bar_wait(&empty[x % g.stages], (x / g.stages) & 1);
             }
         }
         __syncwarp();
     } else if (warp == 1) {
         const uint32_t id = uniform(idesc<T>(128, (uint32_t)g.n_cols, false, QUERY));
-        for (int c = 0; c < chunks; ++c) {
-            const int s = c % g.stages, steps = min(4, g.k_steps - 4 * c);
-            ok = ok && bar_wait_warp(&full[s], (c / g.stages) & 1);
+        int i = 0;          // tiles so far
+        for (int tile = blockIdx.x; ok && tile < g.tiles; tile += gridDim.x, ++i) {
+            ok = i < 2 || bar_wait_warp(&acc_empty[i & 1], (unsigned)((i >> 1) - 1) & 1);
+            const uint32_t d = uniform(tmem + (uint32_t)((i & 1) * g.n_cols));
+            for (int c = 0; c < chunks; ++c) {
+                const int steps = min(4, g.k_steps - 4 * c);
+                ok = ok && bar_wait_warp(&full[s], parity);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t at = base + s * stage_bytes, ad = uniform(desc_k(at)), bd = uniform(QUERY ? desc_mn(at + a_bytes) : desc_k(at + a_bytes));
+                if (elect_one()) {
+                    for (int k = 0; k < steps; ++k) umma_ss(d, ad + k * 2, bd + k * (QUERY ? 2048 / 16 : 2), id, (uint32_t)(c + k > 0));
+                    umma_commit(&empty[s]);
+                    if (c == chunks - 1) umma_commit(&acc_full[i & 1]);
+                }
+                __syncwarp();
+                advance();
+            }
+        }
+        if (!ok) {          // what was issued has to be through before the tensor memory is freed
+            if (elect_one()) umma_commit(&acc_full[i & 1]);
+            __syncwarp();
+            bar_wait_warp(&acc_full[i & 1], (unsigned)(i >> 1) & 1);
+        }
+    } else {
+        if (QUERY) {
+            // The rotation, while the operands travel: half a warp takes (token, eight heads) after (token, eight heads).  (As blocks of
+            // their own behind the products they held as much shared memory as those: a second wave.)
+            const int groups = (g.heads + kRotateHeads - 1) / kRotateHeads;
+            for (int i = blockIdx.x * 8 + ((tid - 64) >> 4); i < g.n_tokens * groups; i += gridDim.x * 8)
+                rotate_heads<T>(g, i / groups, i % groups * kRotateHeads);
+            __syncwarp();
+        }
+        // A tile's sums to shared memory as chunks of 64 columns, the tensor copy's layout, and out.
+        const int row = 32 * (warp & 3) + lane;
+        int i = 0;
+        for (int tile = blockIdx.x; ok && tile < g.tiles; tile += gridDim.x, ++i) {
+            const int col = tile % g.col_blocks * g.n_cols, h = tile / g.col_blocks % g.heads, t0 = tile / g.col_blocks / g.heads * kHeadTokens;
+            ok = bar_wait_warp(&acc_full[i & 1], (unsigned)(i >> 1) & 1);
+            // (every warp comes to these barriers; one whose wait ran out brings its tile's copies to nothing below)
+            if (warp == 2 && elect_one()) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+            bool all;
+            {
+                uint32_t r;
+                asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                             : "=r"(r) : "r"((uint32_t)ok) : "memory");
+                all = r != 0;
+            }
+            ok = all;
             if (!ok) break;
             tc_fence_after();
-            const uint32_t at = base + s * stage_bytes, ad = uniform(desc_k(at)), bd = uniform(QUERY ? desc_mn(at + a_bytes) : desc_k(at + a_bytes));
-            if (elect_one()) {
-                for (int k = 0; k < steps; ++k) umma_ss(tmem, ad + k * 2, bd + k * (QUERY ? 2048 / 16 : 2), id, (uint32_t)(c + k > 0));
-                umma_commit(&empty[s]);
-                if (c == chunks - 1) umma_commit(&done);
-            }
-            __syncwarp();
-        }
-        if (!ok) {      // what was issued has to be through before the tensor memory is freed
-            if (elect_one()) umma_commit(&done);
-            __syncwarp();
-        }
-        bar_wait_warp(&done, 0);
-    } else {
-        // The tile to shared memory, in the place of operands that no MMA reads any more: as chunks of 64 columns, the tensor copy's layout.
-        ok = bar_wait_warp(&done, 0);
-        tc_fence_after();
-        const int row = 32 * (warp & 3) + lane;
-        for (int x = 0; x < g.n_cols / 32; ++x) {
-            uint32_t o[32];
-            tmem_ld_32x32(tmem + 32 * x + ((uint32_t)(32 * (warp & 3)) << 16), o);
-            tmem_ld_wait();
-            unsigned char* to = smem + (base - smem_u32(smem)) + (x >> 1) * kHeadAChunk + row * 128;
+            for (int x = 0; x < g.n_cols / 32; ++x) {
+                uint32_t o[32];
+                tmem_ld_32x32(tmem + (i & 1) * g.n_cols + 32 * x + ((uint32_t)(32 * (warp & 3)) << 16), o);
+                tmem_ld_wait();
+                unsigned char* to = smem + (out_at - smem_u32(smem)) + (x >> 1) * kHeadAChunk + row * 128;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint4 b;
-                b.x = pack2<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1]));
-                b.y = pack2<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
-                b.z = pack2<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
-                b.w = pack2<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
-                *reinterpret_cast<uint4*>(to + ((((x & 1) * 4 + i) ^ (row & 7)) << 4)) = b;
+                for (int y = 0; y < 4; ++y) {
+                    uint4 b;
+                    b.x = pack2<T>(__uint_as_float(o[8 * y]), __uint_as_float(o[8 * y + 1]));
+                    b.y = pack2<T>(__uint_as_float(o[8 * y + 2]), __uint_as_float(o[8 * y + 3]));
+                    b.z = pack2<T>(__uint_as_float(o[8 * y + 4]), __uint_as_float(o[8 * y + 5]));
+                    b.w = pack2<T>(__uint_as_float(o[8 * y + 6]), __uint_as_float(o[8 * y + 7]));
+                    *reinterpret_cast<uint4*>(to + ((((x & 1) * 4 + y) ^ (row & 7)) << 4)) = b;
+                }
             }
+            tc_fence_before();
+            bar_arrive(&acc_empty[i & 1]);
+            proxy_fence();
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (warp == 2 && elect_one()) {
+                for (int x = 0; x < g.n_cols / 64; ++x)
+                    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
+                                 ::"l"(&maps.c), "r"(col + 64 * x), "r"(h), "r"(t0), "r"(out_at + x * kHeadAChunk) : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+            __syncwarp();
         }
-        proxy_fence();
-        tc_fence_before();
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (warp == 2 && ok && elect_one()) {
-            for (int n = 0; n < g.n_cols / 64; ++n)
-                asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
-                             ::"l"(&maps.c), "r"(col + 64 * n), "r"(h), "r"(t0), "r"(base + n * kHeadAChunk) : "memory");
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        }
+        if (warp == 2 && elect_one()) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
     }
     tc_fence_before();
@@ -292,29 +339,27 @@ int launch_heads(HeadArgs g, int dtype, cudaStream_t st) {
     if (!tensor_map_encoder()) return VIB3_ERR_UNSUPPORTED;
     const int tiles = ceil_div(g.n_tokens, kHeadTokens), n_all = QUERY ? kRank : g.dim, k_all = QUERY ? g.dim : kRank;
     g.k_steps = k_all / 16;
-    // The widest columns that still give every SM a CTA (a wider one reads A less often).
-    g.n_cols = 256;
-    while (g.n_cols > 64 && (g.n_cols >= 2 * n_all || tiles * g.heads * ceil_div(n_all, g.n_cols) < sm_count())) g.n_cols /= 2;
+    // 128 columns unless the tiles are then fewer than the SMs (wider ones read A less often).
+    g.n_cols = n_all > 64 && tiles * g.heads * ceil_div(n_all, kHeadMaxCols) >= sm_count() ? kHeadMaxCols : 64;
     g.col_blocks = ceil_div(n_all, g.n_cols);
-    g.product_blocks = tiles * g.heads * g.col_blocks;
-    // All of K in flight at once where 104 KB allow it, so that two CTAs share an SM; at least two stages (a 256-column stage has 48 KB).
-    const int stage = kHeadAChunk + g.n_cols * 128, chunks = ceil_div(k_all, 64);
-    g.stages = chunks < 104 * 1024 / stage ? chunks : 104 * 1024 / stage;
-    if (g.stages > kHeadMaxStages) g.stages = kHeadMaxStages;
-    const int out_bytes = kHeadTokens * g.n_cols * 2, ring = g.stages * stage, smem = 1024 + (ring > out_bytes ? ring : out_bytes);
-    const int e = allow_smem<latent_head_kernel<T, QUERY>>(1024 + 104 * 1024);
+    g.tiles = tiles * g.heads * g.col_blocks;
+    g.a_rows = g.n_tokens >= kHeadTokens ? kHeadTokens : ceil_div(g.n_tokens, 8) * 8;
+    // Two CTAs share an SM.  Behind the ring lie the rows that an MMA of the last stage reads beyond a short A.
+    const int stage = g.a_rows * 128 + g.n_cols * 128;
+    g.stages = kHeadRing / stage < kHeadMaxStages ? kHeadRing / stage : kHeadMaxStages;
+    const int smem = 1024 + kHeadOut + g.stages * stage + kHeadAChunk - g.a_rows * 128;
+    const int e = allow_smem<latent_head_kernel<T, QUERY>>(1024 + kHeadOut + kHeadRing + kHeadAChunk);
     if (e) return e;
     HeadMaps maps;
     const long long width = QUERY ? g.dim + kRope : kRank, out_width = QUERY ? kLatentRow : g.dim;
     // (a dimension of one has no stride that matters)
     const long long at = g.n_tokens > 1 ? g.a_token : width, ah = g.heads > 1 ? g.a_head : width, ot = g.n_tokens > 1 ? g.out_token : out_width,
                     oh = g.heads > 1 ? g.out_head : out_width, wh = g.heads > 1 ? g.w_head : (long long)k_all * n_all;
-    if (!map_3d(&maps.a, dtype, g.a, width, g.heads, g.n_tokens, ah, at, 1, kHeadTokens) ||
+    if (!map_3d(&maps.a, dtype, g.a, width, g.heads, g.n_tokens, ah, at, 1, g.a_rows) ||
         !(QUERY ? map_3d(&maps.b, dtype, g.w, kRank, g.dim, g.heads, kRank, wh, 64, 1) : map_3d(&maps.b, dtype, g.w, kRank, g.dim, g.heads, kRank, wh, g.n_cols, 1)) ||
         !map_3d(&maps.c, dtype, g.out, out_width, g.heads, g.n_tokens, oh, ot, 1, kHeadTokens))
         return VIB3_ERR_SHAPE;
-    const int rotate = QUERY ? ceil_div(g.n_tokens * ceil_div(g.heads, kRotateHeads), kHeadThreads / 16) : 0;
-    return launch_latent(latent_head_kernel<T, QUERY>, dim3((unsigned)(g.product_blocks + rotate)), kHeadThreads, (size_t)smem, st, maps, g);
+    return launch_latent(latent_head_kernel<T, QUERY>, dim3((unsigned)(g.tiles < 2 * sm_count() ? g.tiles : 2 * sm_count())), kHeadThreads, (size_t)smem, st, maps, g);
 }
 
 bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
