@@ -425,3 +425,11 @@ def test_products_at_the_borders_of_their_tiles(cuda_dev, tokens, heads):
     kernels.latent_value(o, v, y)
     a, b = o.double().transpose(0, 1), v.double().transpose(1, 2)
     assert_rounded(y, torch.bmm(a, b).transpose(0, 1), RANK * 2.0 ** -23 * torch.bmm(a.abs(), b.abs()).transpose(0, 1))
+
+
+@pytest.mark.parametrize("others,long,heads", [(0, 30000, 64), (1, 20000, 128), (5, 30000, 64), (30, 40000, 64), (100, 60000, 16), (200, 50000, 64)])
+def test_one_long_sequence_among_short_ones(cuda_dev, others, long, heads):
+    """From two to about 148 parts of one sequence, beside sequences of one part, in every form of the adding launch."""
+    cache, table, lens = paged(cuda_dev, [3 + i % 40 for i in range(others)] + [long], 64, torch.bfloat16, 23)
+    q = torch.randn(lens.numel(), heads, ROW, generator=gen(cuda_dev, 24), device=cuda_dev).to(torch.bfloat16)
+    check_attention(q, cache, table, lens, 0.07)

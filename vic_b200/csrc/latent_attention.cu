@@ -739,26 +739,37 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
 }
 
 // Adds up the parts of the row blocks that several CTAs shared.  The parts lie in the second place of the CTA that begins the block and in
-// the first places of the CTAs after it in its lane.  A unit of work is four rows and 32 of every 128 values (all four 128s, or two of
-// them).  One warp adds up to four parts of a unit; of more parts `team` warps take every team-th each and meet in shared memory.
+// the first places of the CTAs after it in its lane.  A unit of work is four rows and 32 of every 128 values (of all four 128s, or of one).  One warp adds up to four parts of a unit; of more parts `team` warps take every team-th each and meet in shared memory.
 // How large a team, and with it the grid, the launcher chooses by the number of row blocks: a few may have up to 148 parts each,
 // many have about two, and then the blocks beyond the first return at once.
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int y = 16; y; y >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, y));
+    return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int y = 16; y; y >>= 1) v += __shfl_xor_sync(0xffffffffu, v, y);
+    return v;
+}
+
 constexpr int kCombineThreads = 256, kCombineWarps = kCombineThreads / 32, kCombineAlone = 4;
 
 template <typename T, int GN>
 __global__ void __launch_bounds__(kCombineThreads, 2) latent_combine_kernel(const AttentionArgs a, int most) {
-    constexpr int kHalves = 4 / GN, kDepth = 8 / GN;     // parts whose loads are in flight together
+    constexpr int kSplit = 4 / GN, kDepth = 8 / GN;     // parts whose loads are in flight together
     __shared__ float4 sums[kCombineWarps][GN][32];
-    __shared__ float4 weights[kCombineWarps];
+    __shared__ float4 weights[kCombineWarps][kCombineAlone > kMaxGrid / kCombineWarps ? kCombineAlone : (kMaxGrid + kCombineWarps - 1) / kCombineWarps];
+    __shared__ float4 tops[2 * kCombineWarps];
     pdl_enter();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows_all = a.q_len * a.heads;
     const int4 own = a.made_of[blockIdx.y];
     const int parts = own.z, c = own.w, team = parts <= kCombineAlone ? 1 : most;
     const int x = blockIdx.x * kCombineWarps + warp, mate = x & (team - 1), unit = x / team;
-    if (parts < 2 || unit >= a.block_rows * kHalves) return;      // (the same for all warps of a block: team divides their number)
-    const int half = unit % kHalves, u = unit / kHalves;
+    if (parts < 2 || unit >= a.block_rows * kSplit) return;      // (the same for all warps of a block: team divides their number)
+    const int u = unit / kSplit;
     // rows r .. r + 3 of the block, values 128 g + 32 w + lane with g in [g0, g0 + GN)
-    const int w = u & 3, r = (u >> 2) * 4, g0 = GN * half, row0 = own.y * a.block_rows + r;
+    const int w = u & 3, r = (u >> 2) * 4, g0 = GN * (unit % kSplit), row0 = own.y * a.block_rows + r;
     auto place = [&](int k) { return 2 * (c + k * a.lanes) + (k == 0); };
     const float4* src = a.part_o + (w * 64 + (2 * g0 + (r >> 5)) * 8 + ((r & 31) >> 2)) * 32 + lane;
     const float4* ml = reinterpret_cast<const float4*>(a.part_ml + r);     // (m, l) of two rows each
@@ -771,18 +782,44 @@ __global__ void __launch_bounds__(kCombineThreads, 2) latent_combine_kernel(cons
             for (int g = 0; g < GN; ++g) v[i][g] = src[(size_t)place(min(k + i * team, parts - 1)) * (kPartFloats / 4) + g * (2 * 8 * 32)];
     };
     fetch(mate);
+    // The rows' largest reference, the parts' weights relative to it, the sums.  A warp alone does it for itself; a team's block, which has one
+    // group of rows, does it once, a part per thread (every warp for itself: 2000 warps asked for the same lines, 8 us).
     float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+    float4 l = make_float4(0.f, 0.f, 0.f, 0.f), p, q;
+    p.x = p.z = q.x = q.z = -INFINITY;
+    p.y = p.w = q.y = q.w = 0.f;
+    const int mine = team > 1 ? (int)threadIdx.x : lane;
+    if (mine < parts) {
+        p = ml[place(mine) * kMl];
+        q = ml[place(mine) * kMl + 1];
+    }
+    m0 = warp_max(p.x); m1 = warp_max(p.z); m2 = warp_max(q.x); m3 = warp_max(q.z);
+    if (team > 1) {
+        if (lane == 0) tops[warp] = make_float4(m0, m1, m2, m3);
+        __syncthreads();
 #pragma unroll 1
-    for (int k = lane; k < parts; k += 32) {
-        const float4 p = ml[place(k) * kMl], q = ml[place(k) * kMl + 1];
-        m0 = fmaxf(m0, p.x); m1 = fmaxf(m1, p.z); m2 = fmaxf(m2, q.x); m3 = fmaxf(m3, q.z);
+        for (int y = 0; y < (kMaxGrid + 31) / 32; ++y) {
+            const float4 t = tops[y];
+            m0 = fmaxf(m0, t.x); m1 = fmaxf(m1, t.y); m2 = fmaxf(m2, t.z); m3 = fmaxf(m3, t.w);
+        }
     }
-#pragma unroll
-    for (int y = 16; y; y >>= 1) {
-        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, y)); m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, y));
-        m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, y)); m3 = fmaxf(m3, __shfl_xor_sync(0xffffffffu, m3, y));
+    const float4 f = make_float4(weight_of(p.x, m0), weight_of(p.z, m1), weight_of(q.x, m2), weight_of(q.z, m3));
+    l = make_float4(warp_sum(f.x * p.y), warp_sum(f.y * p.w), warp_sum(f.z * q.y), warp_sum(f.w * q.w));
+    float4* const weight = team > 1 ? weights[0] : weights[warp];
+    if (mine < parts) weight[mine] = f;
+    if (team > 1) {
+        if (lane == 0) tops[kCombineWarps + warp] = l;
+        __syncthreads();
+        l = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int y = 0; y < (kMaxGrid + 31) / 32; ++y) {
+            const float4 t = tops[kCombineWarps + y];
+            l.x += t.x; l.y += t.y; l.z += t.z; l.w += t.w;
+        }
+    } else {
+        __syncwarp();
     }
-    float4 o[GN], l = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 o[GN];
 #pragma unroll
     for (int g = 0; g < GN; ++g) o[g] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
@@ -792,13 +829,11 @@ __global__ void __launch_bounds__(kCombineThreads, 2) latent_combine_kernel(cons
         for (int i = 0; i < kDepth; ++i) {
             const int ki = k + i * team;
             if (ki < parts) {
-                const float4 p = ml[place(ki) * kMl], q = ml[place(ki) * kMl + 1];
-                const float f0 = weight_of(p.x, m0), f1 = weight_of(p.z, m1), f2 = weight_of(q.x, m2), f3 = weight_of(q.z, m3);
-                l.x = fmaf(f0, p.y, l.x); l.y = fmaf(f1, p.w, l.y); l.z = fmaf(f2, q.y, l.z); l.w = fmaf(f3, q.w, l.w);
+                const float4 x = weight[ki];
 #pragma unroll
                 for (int g = 0; g < GN; ++g) {
-                    o[g].x = fmaf(f0, v[i][g].x, o[g].x); o[g].y = fmaf(f1, v[i][g].y, o[g].y);
-                    o[g].z = fmaf(f2, v[i][g].z, o[g].z); o[g].w = fmaf(f3, v[i][g].w, o[g].w);
+                    o[g].x = fmaf(x.x, v[i][g].x, o[g].x); o[g].y = fmaf(x.y, v[i][g].y, o[g].y);
+                    o[g].z = fmaf(x.z, v[i][g].z, o[g].z); o[g].w = fmaf(x.w, v[i][g].w, o[g].w);
                 }
             }
         }
@@ -806,7 +841,6 @@ __global__ void __launch_bounds__(kCombineThreads, 2) latent_combine_kernel(cons
     if (team > 1) {
 #pragma unroll
         for (int g = 0; g < GN; ++g) sums[warp][g][lane] = o[g];
-        if (lane == 0) weights[warp] = l;
         __syncthreads();
         if (mate > 0) return;
 #pragma unroll 1
@@ -816,8 +850,6 @@ __global__ void __launch_bounds__(kCombineThreads, 2) latent_combine_kernel(cons
                 const float4 s = sums[warp + y][g][lane];
                 o[g].x += s.x; o[g].y += s.y; o[g].z += s.z; o[g].w += s.w;
             }
-            const float4 s = weights[warp + y];
-            l.x += s.x; l.y += s.y; l.z += s.z; l.w += s.w;
         }
     }
     auto store = [&](int e, float m, float sum, auto value) {
@@ -857,10 +889,10 @@ int launch_attention(const CUtensorMap& map, const AttentionArgs& a, int grid, c
     if (r) return r;
     const long long items = (long long)a.batch * a.lanes * a.blocks_per_lane;
     const int made = a.by_item ? (int)items : grid;
-    const int team = made <= 18 ? 8 : made <= 64 ? 4 : 1, halves = made <= 4 ? 2 : 1;
-    const dim3 blocks((unsigned)(a.block_rows * team * halves / kCombineWarps), (unsigned)made);
-    return halves == 2 ? launch_latent(latent_combine_kernel<T, 2>, blocks, kCombineThreads, 0, st, a, team)
-                       : launch_latent(latent_combine_kernel<T, 4>, blocks, kCombineThreads, 0, st, a, team);
+    const int team = made <= 18 ? 8 : made <= 64 ? 4 : 2, split = made <= 4 ? 4 : 1;
+    const dim3 blocks((unsigned)(a.block_rows * team * split / kCombineWarps), (unsigned)made);
+    return split == 4 ? launch_latent(latent_combine_kernel<T, 1>, blocks, kCombineThreads, 0, st, a, team)
+                      : launch_latent(latent_combine_kernel<T, 4>, blocks, kCombineThreads, 0, st, a, team);
 }
 
 }  // namespace
