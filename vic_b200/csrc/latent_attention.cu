@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
                     float4* out = a.part_o + (size_t)part * (kPartFloats / 4) + w * (8 * 8 * 32) + lane;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        out[(x * 8 + i) * 32] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                        if (32 * (x & 1) + 4 * i < n) out[(x * 8 + i) * 32] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
                                                             __uint_as_float(o[4 * i + 3]));
                 }
             }
@@ -770,6 +770,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2) latent_combine_kernel(cons
     const int u = unit / kSplit;
     // rows r .. r + 3 of the block, values 128 g + 32 w + lane with g in [g0, g0 + GN)
     const int w = u & 3, r = (u >> 2) * 4, g0 = GN * (unit % kSplit), row0 = own.y * a.block_rows + r;
+    if (row0 >= rows_all) return;              // (a block whose warps meet has one group of rows)
     auto place = [&](int k) { return 2 * (c + k * a.lanes) + (k == 0); };
     const float4* src = a.part_o + (w * 64 + (2 * g0 + (r >> 5)) * 8 + ((r & 31) >> 2)) * 32 + lane;
     const float4* ml = reinterpret_cast<const float4*>(a.part_ml + r);     // (m, l) of two rows each
@@ -947,7 +948,7 @@ extern "C" int vib3_launch_latent_attention_paged(const void* q, long long q_tok
     const long long rows = (long long)q_len * heads, most_tiles = ((long long)max_pages_per_seq * page_size + kTileKeys - 1) / kTileKeys;
     // Half row blocks where the whole ones would leave half of the SMs without work: the cache is then read twice (from L2), the
     // results of a CTA, 128 KB at 30 bytes per cycle, are halved.
-    a.block_rows = rows > 32 && (rows + kTileRows - 1) / kTileRows * batch * most_tiles <= sms ? kTileRows / 2 : kTileRows;
+    a.block_rows = rows <= 32 || (rows + kTileRows - 1) / kTileRows * batch * most_tiles <= sms ? kTileRows / 2 : kTileRows;
     const int blocks = (int)((rows + a.block_rows - 1) / a.block_rows);
     a.lanes = blocks <= 8 ? blocks : 1;
     a.blocks_per_lane = blocks / a.lanes;
