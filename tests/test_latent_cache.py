@@ -1,0 +1,74 @@
+"""The host side of the latent cache: pages, slots and positions of a step's tokens (no GPU needed)."""
+import pytest
+import torch
+
+
+def make(**k):
+    from vic_b200.attention import LatentCache
+    a = dict(layers=2, pages=6, page_size=8, max_sequences=3, max_pages=4, dtype=torch.bfloat16, device="cpu", max_tokens=64)
+    a.update(k)
+    return LatentCache(**a)
+
+
+def slots_of(cache, b, lo, hi):
+    return [int(cache.table[b, p // cache.page_size]) * cache.page_size + p % cache.page_size for p in range(lo, hi)]
+
+
+def test_steps_give_every_token_a_slot_of_its_own():
+    c = make()
+    c.begin_step([5, 0, 9])                                     # a chunk of 9 rows per sequence, the shorter ones padded in front
+    assert c.lens.tolist() == [5, 0, 9]
+    assert c.slots[:27].tolist() == [-1] * 4 + slots_of(c, 0, 0, 5) + [-1] * 9 + slots_of(c, 2, 0, 9)
+    assert c.positions[:27].tolist() == [0] * 4 + list(range(5)) + [0] * 9 + list(range(9))
+    seen = set(slots_of(c, 0, 0, 5) + slots_of(c, 2, 0, 9))
+    assert len(seen) == 14
+    for step in range(4):
+        c.begin_step([1, 1, 0])
+        assert c.slots[:3].tolist() == slots_of(c, 0, 5 + step, 6 + step) + slots_of(c, 1, step, step + 1) + [-1]
+        assert c.positions[:3].tolist() == [5 + step, step, 0]
+        new = [s for s in c.slots[:3].tolist() if s >= 0]
+        assert not seen & set(new)
+        seen |= set(new)
+    assert c.lens.tolist() == [9, 4, 9]
+
+
+def test_a_full_cache_refuses_the_step_and_stays_as_it_was():
+    from vic_b200.lib import Vib3Error
+    c = make()
+    c.begin_step([16, 16, 8], q_len=16)
+    before = (c.lens.tolist(), c.table.tolist(), list(c._free))
+    with pytest.raises(Vib3Error):
+        c.begin_step([1, 1, 0])                                 # two pages wanted, one left
+    with pytest.raises(ValueError):
+        c.begin_step([1, 1])
+    with pytest.raises(ValueError):
+        c.begin_step([2, 0, 0], q_len=1)
+    with pytest.raises(ValueError):
+        c.begin_step([-1, 0, 0], q_len=1)
+    with pytest.raises(ValueError):
+        c.begin_step([30, 0, 0])
+    assert before == (c.lens.tolist(), c.table.tolist(), list(c._free)) and c.host_lens == [16, 16, 8]
+    c.begin_step([1, 0, 0])
+    with pytest.raises(Vib3Error):
+        c.begin_step([0, 1, 0])
+    c.release(2)
+    c.begin_step([0, 1, 1], q_len=1) if len(c._free) > 1 else c.begin_step([0, 1, 0], q_len=1)
+    assert c.host_lens[1] == 17
+
+
+def test_a_sequence_has_no_more_pages_than_its_table():
+    from vic_b200.lib import Vib3Error
+    c = make(pages=100, max_tokens=200)
+    c.begin_step([32, 0, 0])
+    with pytest.raises(Vib3Error):
+        c.begin_step([1, 0, 0])
+    c.release(0)
+    c.begin_step([1, 0, 0])
+    assert c.lens.tolist() == [1, 0, 0]
+
+
+def test_bad_layouts_are_refused():
+    with pytest.raises(ValueError):
+        make(page_size=12)
+    with pytest.raises(ValueError):
+        make(max_tokens=2)

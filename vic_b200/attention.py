@@ -1,0 +1,136 @@
+"""The latent-attention sublayer of a decode layer, and the layer made of it and the MoE sublayer.
+
+The reference runs this sublayer token by token over a flat cache (src/runtime/attention.rs; kernels cuda/src/kernels.cu:1570-1740).
+Here the newest tokens of a batch go through it together: ``LatentCache`` keeps the paged rows of every layer and, per step, where the new
+tokens' rows go; ``LatentAttention`` is one layer's weights and its launches; ``DecodeLayer`` puts it before MoeDecoder or
+GroupedDecoder.  Projections from and to the hidden state are plain library products.  After ``LatentCache.begin_step`` (host) everything
+is device work on fixed buffers and can be captured into a CUDA graph."""
+from __future__ import annotations
+
+from typing import List, Optional, Sequence
+
+import torch
+
+from . import kernels
+from .core_types import LatentShape
+from .kernels import LATENT_RANK, LATENT_ROPE, LATENT_ROW
+from .lib import Vib3Error
+
+
+class LatentCache:
+    """Paged latent rows of ``layers`` layers for up to ``max_sequences`` sequences of up to ``max_pages`` pages each.  One page table
+    serves all layers.  Device buffers of a step (fixed addresses): ``table``, ``lens``, ``positions`` and ``slots``."""
+
+    def __init__(self, layers: int, pages: int, page_size: int, max_sequences: int, max_pages: int, dtype: torch.dtype, device,
+                 max_tokens: int = 128):
+        if page_size <= 0 or page_size % 8:
+            raise ValueError("page_size: a positive multiple of 8")
+        if max_tokens < max_sequences:
+            raise ValueError("max_tokens: at least one token per sequence")
+        self.page_size, self.max_sequences, self.max_pages, self.max_tokens = page_size, max_sequences, max_pages, max_tokens
+        self.rows = torch.zeros(layers, pages, page_size, LATENT_ROW, dtype=dtype, device=device)
+        self.table = torch.zeros(max_sequences, max_pages, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(max_sequences, dtype=torch.int32, device=device)
+        self.positions = torch.zeros(max_tokens, dtype=torch.int32, device=device)
+        self.slots = torch.full((max_tokens,), -1, dtype=torch.int64, device=device)
+        self.host_lens: List[int] = [0] * max_sequences
+        self._pages_of: List[List[int]] = [[] for _ in range(max_sequences)]
+        self._free = list(range(pages - 1, -1, -1))
+
+    def begin_step(self, new_tokens: Sequence[int], q_len: Optional[int] = None) -> None:
+        """Sequence b gets new_tokens[b] tokens (0: it takes no part): pages for them, their positions and slots, the lengths with
+        them.  A step's rows are q_len (default: the largest count) per sequence, the new tokens last; the rows before them are padding."""
+        if len(new_tokens) != self.max_sequences:
+            raise ValueError(f"{self.max_sequences} counts expected")
+        q_len = max(new_tokens) if q_len is None else q_len
+        if min(new_tokens) < 0 or max(new_tokens) > q_len or q_len * self.max_sequences > self.max_tokens:
+            raise ValueError("counts have to lie in 0 .. q_len, and q_len * sequences within max_tokens")
+        need = [-(-(n + k) // self.page_size) for n, k in zip(self.host_lens, new_tokens)]
+        if max(need) > self.max_pages or sum(max(0, n - len(p)) for n, p in zip(need, self._pages_of)) > len(self._free):
+            raise Vib3Error("latent cache: no page left for the step's tokens", -8)
+        positions, slots = [], []
+        for b, k in enumerate(new_tokens):
+            own, first = self._pages_of[b], self.host_lens[b]
+            while len(own) < need[b]:
+                own.append(self._free.pop())
+            pad = q_len - k
+            positions += [0] * pad + list(range(first, first + k))
+            slots += [-1] * pad + [own[p // self.page_size] * self.page_size + p % self.page_size for p in range(first, first + k)]
+            self.host_lens[b] = first + k
+        table = [own + [0] * (self.max_pages - len(own)) for own in self._pages_of]
+        n = len(positions)
+        self.positions[:n].copy_(torch.tensor(positions, dtype=torch.int32))
+        self.slots[:n].copy_(torch.tensor(slots, dtype=torch.int64))
+        self.table.copy_(torch.tensor(table, dtype=torch.int32))
+        self.lens.copy_(torch.tensor(self.host_lens, dtype=torch.int32))
+
+    def release(self, sequence: int) -> None:
+        """Forget a sequence; its pages may go to others."""
+        self._free += self._pages_of[sequence][::-1]
+        self._pages_of[sequence] = []
+        self.host_lens[sequence] = 0
+
+
+class LatentAttention:
+    """One layer: x [T, hidden] -> output [T, hidden], T = sequences * q_len rows in the cache's order.
+
+    ``w_q`` [heads * (nope + 64), hidden], ``w_kv`` [576, hidden], ``kv_norm`` [512], ``kv_b`` [heads, nope + value, 512] (the heads' key
+    and value matrices), ``w_o`` [hidden, heads * value]; one dtype, fp16 or bf16."""
+
+    def __init__(self, shape: LatentShape, w_q: torch.Tensor, w_kv: torch.Tensor, kv_norm: torch.Tensor, kv_b: torch.Tensor,
+                 w_o: torch.Tensor, max_tokens: int = 128, workspace: Optional[torch.Tensor] = None):
+        dev, dt, H = w_q.device, w_q.dtype, shape.heads
+        if w_q.shape != (H * (shape.nope + LATENT_ROPE), shape.hidden) or w_kv.shape != (LATENT_ROW, shape.hidden) or kv_norm.shape != (LATENT_RANK,) or \
+                kv_b.shape != (H, shape.nope + shape.value, LATENT_RANK) or w_o.shape != (shape.hidden, H * shape.value):
+            raise ValueError("weights do not have the layer's shape")
+        self.shape, self.max_tokens = shape, max_tokens
+        self.w_q, self.w_kv, self.kv_norm, self.kv_b, self.w_o = w_q, w_kv, kv_norm, kv_b, w_o
+        self.inv_freq = shape.rope_theta ** (-torch.arange(0, LATENT_ROPE, 2, dtype=torch.float64, device=dev) / LATENT_ROPE)
+        self.q_in = torch.zeros(max_tokens, H * (shape.nope + LATENT_ROPE), dtype=dt, device=dev)
+        self.kv_in = torch.zeros(max_tokens, LATENT_ROW, dtype=dt, device=dev)
+        self.q = torch.zeros(max_tokens, H, LATENT_ROW, dtype=dt, device=dev)
+        self.o = torch.zeros(max_tokens, H, LATENT_RANK, dtype=dt, device=dev)
+        self.v = torch.zeros(max_tokens, H, shape.value, dtype=dt, device=dev)
+        self.out = torch.zeros(max_tokens, shape.hidden, dtype=dt, device=dev)
+        self.status = torch.zeros(1, dtype=torch.int32, device=dev)
+        # layers that run one after another may share it
+        self.workspace = torch.empty(kernels.latent_attention_workspace_bytes(), dtype=torch.uint8, device=dev) if workspace is None else workspace
+
+    def forward(self, x: torch.Tensor, cache: LatentCache, layer: int) -> torch.Tensor:
+        """The step that ``cache.begin_step`` laid out.  Returns a view of ``self.out``."""
+        sh, T = self.shape, x.shape[0]
+        if T > self.max_tokens or T % cache.max_sequences:
+            raise ValueError("x: a row for each of the step's sequences * q_len tokens expected")
+        rows, pos = cache.rows[layer], cache.positions[:T]
+        torch.matmul(x, self.w_kv.t(), out=self.kv_in[:T])
+        torch.matmul(x, self.w_q.t(), out=self.q_in[:T])
+        kernels.latent_append(self.kv_in[:T], self.kv_norm, sh.eps, pos, cache.slots[:T], self.inv_freq, rows, status=self.status)
+        kernels.latent_query(self.q_in[:T].view(T, sh.heads, sh.nope + LATENT_ROPE), self.kv_b[:, :sh.nope], pos, self.inv_freq, self.q[:T])
+        kernels.latent_attention(self.q[:T], rows, cache.table, cache.lens, sh.scale, self.o[:T], workspace=self.workspace, status=self.status)
+        kernels.latent_value(self.o[:T], self.kv_b[:, sh.nope:], self.v[:T])
+        torch.matmul(self.v[:T].view(T, sh.heads * sh.value), self.w_o.t(), out=self.out[:T])
+        return self.out[:T]
+
+
+class DecodeLayer:
+    """h += attention(norm(h)), h += moe(norm(h)) for a step's rows: ``moe`` is a MoeDecoder (one row) or a GroupedDecoder."""
+
+    def __init__(self, attention: LatentAttention, moe, layer: int, attention_norm: torch.Tensor, moe_norm: torch.Tensor, eps: float = 1e-6):
+        self.attention, self.moe, self.layer = attention, moe, layer
+        self.attention_norm, self.moe_norm, self.eps = attention_norm, moe_norm, eps
+        self.x = torch.zeros(attention.max_tokens, attention.shape.hidden, dtype=attention.w_q.dtype, device=attention.w_q.device)
+
+    def forward(self, h: torch.Tensor, cache: LatentCache) -> torch.Tensor:
+        """h [T, hidden] fp32, updated in place."""
+        T = h.shape[0]
+        x = self.x[:T]
+        kernels.residual_rms_norm(h, None, self.attention_norm, self.eps, x)
+        delta = self.attention.forward(x, cache, self.layer)
+        kernels.residual_rms_norm(h, delta, self.moe_norm, self.eps, x, early_dependents=True)
+        if hasattr(self.moe, "max_tokens"):
+            self.moe.forward(self.layer, x, out=h, accumulate=True, hold=True)
+        elif T == 1:
+            self.moe.forward_layer(self.layer, x[0], out=h[0], accumulate=True, hold=True)
+        else:
+            raise ValueError("MoeDecoder takes one row; GroupedDecoder takes several")
+        return h

@@ -108,3 +108,23 @@ class MoeShape:
 MIXTRAL = MoeShape("mixtral-8x7b", 4096, 14336, 8, 2, 0, SCORING_SOFTMAX, 1.0, True)
 # Kimi-K2.5-shape layer (types.rs:30-68): sigmoid scoring, top-8 renormalised, x2.827, one shared expert
 KIMI = MoeShape("kimi-k2.5", 7168, 2048, 384, 8, 1, SCORING_SIGMOID, 2.827, True)
+
+
+@dataclass(frozen=True)
+class LatentShape:
+    """One latent-attention layer's sizes.  The cache row is fixed: 512 latent and 64 position values (what the kernels take)."""
+    name: str
+    hidden: int
+    heads: int
+    nope: int                # width of a head's query part without positions
+    value: int               # width of a head's output
+    rope_theta: float
+    eps: float
+
+    @property
+    def scale(self) -> float:
+        return (self.nope + 64) ** -0.5
+
+
+# The attention sublayer that goes with KIMI: 64 heads of 128 + 64 and 128 over a latent of 512
+KIMI_LATENT = LatentShape("kimi-k2.5", 7168, 64, 128, 128, 50000.0, 1e-6)

@@ -320,15 +320,22 @@ _X_CODES = {torch.float32: X_F32, torch.float16: X_F16, torch.bfloat16: X_BF16}
 _I32, _I64, _F32, _F64 = torch.int32, torch.int64, torch.float32, torch.float64
 
 
-def _device() -> int:
-    """The current device.  The operands have to lie on it: a launch on another one would read through a foreign context."""
+_current_device, _current_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_latent = None       # the library's latent launchers, once the device is there
+
+
+def _bind_latent():
+    """(append, query, value, attention): the launchers, looked up once.  CUDA is initialised here, not by every call."""
+    global _latent
     if not torch.cuda.is_initialized():
         torch.cuda.init()
-    return torch._C._cuda_getDevice()
+    h = lib()
+    _latent = (h.vib3_launch_latent_append_paged, h.vib3_launch_latent_query, h.vib3_launch_latent_value, h.vib3_launch_latent_attention_paged)
+    return _latent
 
 
 def _foreign(*tensors) -> ValueError:
-    return ValueError(f"operands have to be on the current device (cuda:{_device()}), got {[str(t.device) for t in tensors if t is not None]}")
+    return ValueError(f"operands have to be on the current device (cuda:{_current_device()}), got {[str(t.device) for t in tensors if t is not None]}")
 
 
 def latent_append(kv: torch.Tensor, norm_weight: Optional[torch.Tensor], eps: float, positions: torch.Tensor, slots: torch.Tensor,
@@ -354,13 +361,15 @@ def latent_append(kv: torch.Tensor, norm_weight: Optional[torch.Tensor], eps: fl
         raise ValueError("inv_freq: contiguous float64 [32] expected")
     if norm_weight is not None and (norm_weight.shape != (LATENT_RANK,) or norm_weight.dtype != dt or not norm_weight.is_contiguous()):
         raise ValueError("norm_weight: contiguous [512] of the cache's dtype expected")
-    if not (_device() == kv.get_device() == cache.get_device() == slots.get_device() == positions.get_device() == inv_freq.get_device()
+    launch = (_latent or _bind_latent())[0]
+    dev = _current_device()     # (a launch on another one would read through a foreign context)
+    if not (dev == kv.get_device() == cache.get_device() == slots.get_device() == positions.get_device() == inv_freq.get_device()
             == (kv if norm_weight is None else norm_weight).get_device() == (kv if status is None else status).get_device()):
         raise _foreign(kv, cache, slots, positions, inv_freq, norm_weight, status)
-    err = lib().vib3_launch_latent_append_paged(
+    err = launch(
         kv.data_ptr(), code, kv_stride, 0 if norm_weight is None else norm_weight.data_ptr(), eps, positions.data_ptr(), slots.data_ptr(),
         inv_freq.data_ptr(), rope_scale, 1 if pairs else 0, T, cache.data_ptr(), _X_CODES[dt], pages, page, page_stride, row_stride,
-        0 if status is None else status.data_ptr(), _stream(stream))
+        0 if status is None else status.data_ptr(), _current_stream(dev) if stream is None else stream)
     if err:
         check("latent_append", err)
 
@@ -385,11 +394,13 @@ def latent_query(q: torch.Tensor, w_uk: torch.Tensor, positions: torch.Tensor, i
         raise ValueError("inv_freq: contiguous float64 [32] expected")
     if (dt != torch.bfloat16 and dt != torch.float16) or w_uk.dtype != dt or out.dtype != dt:
         raise ValueError("one dtype, fp16 or bf16, expected")
-    if not (_device() == q.get_device() == w_uk.get_device() == positions.get_device() == inv_freq.get_device() == out.get_device()):
+    launch = (_latent or _bind_latent())[1]
+    dev = _current_device()     # (a launch on another one would read through a foreign context)
+    if not (dev == q.get_device() == w_uk.get_device() == positions.get_device() == inv_freq.get_device() == out.get_device()):
         raise _foreign(q, w_uk, positions, inv_freq, out)
-    err = lib().vib3_launch_latent_query(
+    err = launch(
         q.data_ptr(), q0, q1, w_uk.data_ptr(), w0, positions.data_ptr(), inv_freq.data_ptr(), rope_scale, 1 if pairs else 0, out.data_ptr(),
-        o0, o1, T, H, nope, _X_CODES[dt], _stream(stream))
+        o0, o1, T, H, nope, _X_CODES[dt], _current_stream(dev) if stream is None else stream)
     if err:
         check("latent_query", err)
 
@@ -409,10 +420,12 @@ def latent_value(o: torch.Tensor, w_uv: torch.Tensor, out: torch.Tensor, stream:
         raise ValueError("out: [T, H, value] with contiguous rows expected")
     if (dt != torch.bfloat16 and dt != torch.float16) or w_uv.dtype != dt or out.dtype != dt:
         raise ValueError("one dtype, fp16 or bf16, expected")
-    if not (_device() == o.get_device() == w_uv.get_device() == out.get_device()):
+    launch = (_latent or _bind_latent())[2]
+    dev = _current_device()     # (a launch on another one would read through a foreign context)
+    if not (dev == o.get_device() == w_uv.get_device() == out.get_device()):
         raise _foreign(o, w_uv, out)
-    err = lib().vib3_launch_latent_value(o.data_ptr(), i0, i1, w_uv.data_ptr(), w0, out.data_ptr(), o0, o1, T, H, value, _X_CODES[dt],
-                                         _stream(stream))
+    err = launch(o.data_ptr(), i0, i1, w_uv.data_ptr(), w0, out.data_ptr(), o0, o1, T, H, value, _X_CODES[dt],
+                                         _current_stream(dev) if stream is None else stream)
     if err:
         check("latent_value", err)
 
@@ -451,13 +464,15 @@ def latent_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Ten
         raise ValueError("one dtype, fp16 or bf16, expected")
     if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise ValueError("workspace: contiguous uint8 expected")
-    if not (_device() == q.get_device() == cache.get_device() == page_table.get_device() == seq_lens.get_device() == out.get_device()
+    launch = (_latent or _bind_latent())[3]
+    dev = _current_device()     # (a launch on another one would read through a foreign context)
+    if not (dev == q.get_device() == cache.get_device() == page_table.get_device() == seq_lens.get_device() == out.get_device()
             == workspace.get_device() == (q if lse is None else lse).get_device() == (q if status is None else status).get_device()):
         raise _foreign(q, cache, page_table, seq_lens, out, workspace, lse, status)
-    err = lib().vib3_launch_latent_attention_paged(
+    err = launch(
         q.data_ptr(), q0, q1, cache.data_ptr(), pages, page, c0, c1, page_table.data_ptr(), t0, max_pages, seq_lens.data_ptr(), B, q_len, H,
         scale, _X_CODES[dt], out.data_ptr(), o0, o1, 0 if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.numel(),
-        0 if status is None else status.data_ptr(), _stream(stream))
+        0 if status is None else status.data_ptr(), _current_stream(dev) if stream is None else stream)
     if err:
         check("latent_attention", err)
 
