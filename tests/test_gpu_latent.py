@@ -433,3 +433,36 @@ def test_one_long_sequence_among_short_ones(cuda_dev, others, long, heads):
     cache, table, lens = paged(cuda_dev, [3 + i % 40 for i in range(others)] + [long], 64, torch.bfloat16, 23)
     q = torch.randn(lens.numel(), heads, ROW, generator=gen(cuda_dev, 24), device=cuda_dev).to(torch.bfloat16)
     check_attention(q, cache, table, lens, 0.07)
+
+
+@pytest.mark.parametrize("B,n,heads,q_len", [(64, 2500, 64, 1), (200, 500, 16, 1), (30, 3000, 64, 2), (120, 700, 128, 1)])
+def test_shared_sequences_give_the_same_bits_every_time(cuda_dev, B, n, heads, q_len):
+    """The CTAs that share a sequence meet in whatever order; who adds up the parts must not show.  A graph's replays too."""
+    from vic_b200 import kernels
+    cache, table, lens = paged(cuda_dev, [n - (37 * b) % 400 for b in range(B)], 64, torch.bfloat16, 25)
+    q = torch.randn(B * q_len, heads, ROW, generator=gen(cuda_dev, 26), device=cuda_dev).to(torch.bfloat16)
+    ws = torch.randint(0, 256, (kernels.latent_attention_workspace_bytes(),), dtype=torch.uint8, device=cuda_dev)
+    want, wlse = check_attention(q, cache, table, lens, 0.07, workspace=ws)
+    out, lse = torch.empty_like(want), torch.empty_like(wlse)
+    load = torch.randn(4096, 4096, device=cuda_dev)
+    side = torch.cuda.Stream()
+    for i in range(60):
+        out.fill_(7.0)
+        if i % 3 == 1:      # another stream's work takes SMs away meanwhile
+            with torch.cuda.stream(side):
+                load = torch.tanh(load @ load)
+        kernels.latent_attention(q, cache, table, lens, 0.07, out, lse, workspace=ws)
+        assert torch.equal(out, want) and torch.equal(lse, wlse), i
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kernels.latent_attention(q, cache, table, lens, 0.07, out, lse, workspace=ws)
+    for i in range(20):
+        out.fill_(7.0)
+        graph.replay()
+        assert torch.equal(out, want) and torch.equal(lse, wlse), i
+    lens.sub_(100)          # (the replays read the lengths again)
+    graph.replay()
+    again = torch.empty_like(out)
+    kernels.latent_attention(q, cache, table, lens, 0.07, again, workspace=ws)
+    assert torch.equal(out, again)

@@ -105,11 +105,12 @@ __global__ void __launch_bounds__(kAppendWarps * 32) latent_append_kernel(Append
 // These products are bound by their bytes: with one token the head matrices are read for two flops per value, with 512 a query's
 // result rows are most of the traffic (and the tensor pipe is busy for a fifth of the time).  So what counts is many bytes in flight
 // with few instructions (warp-level MMAs fed by 16-byte copies spent their time on addresses: 500 queries of 64 heads in 32 us), and that
-// reads and writes overlap: two CTAs per SM take tile after tile, the ring runs on across them, and of two accumulators one is
-// stored while the other is filled (a CTA per tile, all of them loading and then all of them storing: 16.7 us).
-constexpr int kHeadTokens = 128, kHeadAChunk = kHeadTokens * 128, kHeadMaxStages = 8, kHeadMaxCols = 128;
-constexpr int kHeadOut = kHeadTokens * kHeadMaxCols * 2, kHeadRing = 64 * 1024;
-constexpr int kHeadThreads = 192;          // copies, MMAs, four warps for the results
+// reads and writes overlap: a CTA per SM takes tile after tile, the ring (160 KB) runs ahead across them, and of two accumulators one is
+// stored while the other is filled.  (A CTA per tile, all of them loading and then all of them storing: 16.7 us; two CTAs per SM with a
+// third of the ring each, where a tile's loads waited for the tile before: 15.8.)
+constexpr int kHeadTokens = 128, kHeadAChunk = kHeadTokens * 128, kHeadMaxStages = 12, kHeadMaxCols = 128;
+constexpr int kHeadOut = kHeadTokens * kHeadMaxCols * 2, kHeadRing = 160 * 1024;   // (two such tiles)
+constexpr int kHeadThreads = 320;          // copies, MMAs, four warps for the results, four for the rotation
 
 struct HeadMaps {
     CUtensorMap a, b, c;
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(kHeadThreads) latent_head_kernel(const __grid_
     __shared__ uint32_t tmem_at;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     // (the swizzle goes by the address, and the static arrays stand before the dynamic memory)
-    const uint32_t out_at = (smem_u32(smem) + 1023u) & ~1023u, base = out_at + kHeadOut;
+    const uint32_t out_at = (smem_u32(smem) + 1023u) & ~1023u, base = out_at + 2 * kHeadOut;
     // (A's rows behind the copied ones are whatever lies there: the MMA reads them, and their sums are not stored)
     const uint32_t a_bytes = (uint32_t)g.a_rows * 128, b_bytes = (uint32_t)g.n_cols * 128, stage_bytes = a_bytes + b_bytes;
     const int chunks = (g.k_steps + 3) >> 2;
@@ -264,23 +265,24 @@ __global__ void __launch_bounds__(kHeadThreads) latent_head_kernel(const __grid_
             __syncwarp();
             bar_wait_warp(&acc_full[i & 1], (unsigned)(i >> 1) & 1);
         }
-    } else {
+    } else if (warp >= 6) {
         if (QUERY) {
-            // The rotation, while the operands travel: half a warp takes (token, eight heads) after (token, eight heads).  (As blocks of
-            // their own behind the products they held as much shared memory as those: a second wave.)
+            // The rotation beside the products: half a warp takes (token, eight heads) after (token, eight heads).  (As blocks of their own they
+            // held as much shared memory as a product's; by the warps of the results, before those, four rounds of it took 10000 cycles.)
             const int groups = (g.heads + kRotateHeads - 1) / kRotateHeads;
-            for (int i = blockIdx.x * 8 + ((tid - 64) >> 4); i < g.n_tokens * groups; i += gridDim.x * 8)
+            for (int i = blockIdx.x * 8 + ((tid - 192) >> 4); i < g.n_tokens * groups; i += gridDim.x * 8)
                 rotate_heads<T>(g, i / groups, i % groups * kRotateHeads);
             __syncwarp();
         }
+    } else {
         // A tile's sums to shared memory as chunks of 64 columns, the tensor copy's layout, and out.
         const int row = 32 * (warp & 3) + lane;
         int i = 0;
         for (int tile = blockIdx.x; ok && tile < g.tiles; tile += gridDim.x, ++i) {
             const int col = tile % g.col_blocks * g.n_cols, h = tile / g.col_blocks % g.heads, t0 = tile / g.col_blocks / g.heads * kHeadTokens;
             ok = bar_wait_warp(&acc_full[i & 1], (unsigned)(i >> 1) & 1);
-            // (every warp comes to these barriers; one whose wait ran out brings its tile's copies to nothing below)
-            if (warp == 2 && elect_one()) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            // (the copies of the tile two before have read their place; every warp comes to these barriers)
+            if (warp == 2 && elect_one()) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
             __syncwarp();
             bool all;
             {
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(kHeadThreads) latent_head_kernel(const __grid_
                 uint32_t o[32];
                 tmem_ld_32x32(tmem + (i & 1) * g.n_cols + 32 * x + ((uint32_t)(32 * (warp & 3)) << 16), o);
                 tmem_ld_wait();
-                unsigned char* to = smem + (out_at - smem_u32(smem)) + (x >> 1) * kHeadAChunk + row * 128;
+                unsigned char* to = smem + (out_at - smem_u32(smem)) + (i & 1) * kHeadOut + (x >> 1) * kHeadAChunk + row * 128;
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
                     uint4 b;
@@ -314,7 +316,7 @@ __global__ void __launch_bounds__(kHeadThreads) latent_head_kernel(const __grid_
             if (warp == 2 && elect_one()) {
                 for (int x = 0; x < g.n_cols / 64; ++x)
                     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
-                                 ::"l"(&maps.c), "r"(col + 64 * x), "r"(h), "r"(t0), "r"(out_at + x * kHeadAChunk) : "memory");
+                                 ::"l"(&maps.c), "r"(col + 64 * x), "r"(h), "r"(t0), "r"(out_at + (i & 1) * kHeadOut + x * kHeadAChunk) : "memory");
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
             __syncwarp();
@@ -344,11 +346,11 @@ int launch_heads(HeadArgs g, int dtype, cudaStream_t st) {
     g.col_blocks = ceil_div(n_all, g.n_cols);
     g.tiles = tiles * g.heads * g.col_blocks;
     g.a_rows = g.n_tokens >= kHeadTokens ? kHeadTokens : ceil_div(g.n_tokens, 8) * 8;
-    // Two CTAs share an SM.  Behind the ring lie the rows that an MMA of the last stage reads beyond a short A.
-    const int stage = g.a_rows * 128 + g.n_cols * 128;
-    g.stages = kHeadRing / stage < kHeadMaxStages ? kHeadRing / stage : kHeadMaxStages;
-    const int smem = 1024 + kHeadOut + g.stages * stage + kHeadAChunk - g.a_rows * 128;
-    const int e = allow_smem<latent_head_kernel<T, QUERY>>(1024 + kHeadOut + kHeadRing + kHeadAChunk);
+    // Behind the ring lie the rows that an MMA of the last stage reads beyond a short A.
+    const int stage = g.a_rows * 128 + g.n_cols * 128, tail = kHeadAChunk - g.a_rows * 128;
+    g.stages = (kHeadRing - tail) / stage < kHeadMaxStages ? (kHeadRing - tail) / stage : kHeadMaxStages;
+    const int smem = 1024 + 2 * kHeadOut + g.stages * stage + tail;
+    const int e = allow_smem<latent_head_kernel<T, QUERY>>(1024 + 2 * kHeadOut + kHeadRing);
     if (e) return e;
     HeadMaps maps;
     const long long width = QUERY ? g.dim + kRope : kRank, out_width = QUERY ? kLatentRow : g.dim;
@@ -359,7 +361,7 @@ int launch_heads(HeadArgs g, int dtype, cudaStream_t st) {
         !(QUERY ? map_3d(&maps.b, dtype, g.w, kRank, g.dim, g.heads, kRank, wh, 64, 1) : map_3d(&maps.b, dtype, g.w, kRank, g.dim, g.heads, kRank, wh, g.n_cols, 1)) ||
         !map_3d(&maps.c, dtype, g.out, out_width, g.heads, g.n_tokens, oh, ot, 1, kHeadTokens))
         return VIB3_ERR_SHAPE;
-    return launch_latent(latent_head_kernel<T, QUERY>, dim3((unsigned)(g.tiles < 2 * sm_count() ? g.tiles : 2 * sm_count())), kHeadThreads, (size_t)smem, st, maps, g);
+    return launch_latent(latent_head_kernel<T, QUERY>, dim3((unsigned)(g.tiles < sm_count() ? g.tiles : sm_count())), kHeadThreads, (size_t)smem, st, maps, g);
 }
 
 bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
