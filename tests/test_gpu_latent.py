@@ -254,7 +254,7 @@ def paged(dev, lens, page, dtype, seed, spare=3, fill=None, row_pad=0):
     ([1], 1, 1, 64, "bf16"), ([1, 2, 0, 3], 1, 64, 16, "bf16"), ([63, 64, 65, 127, 128, 129], 1, 64, 64, "fp16"),
     ([40], 1, 8, 8, "fp16"), ([700, 31, 1999], 1, 16, 24, "bf16"), ([4001], 1, 64, 64, "bf16"), ([300, 5], 1, 128, 128, "fp16"),
     ([513, 2000], 1, 101, 40, "bf16"), ([3, 0, 700], 5, 16, 16, "fp16"), ([1000, 66], 9, 64, 64, "bf16"), ([129], 129, 3, 32, "bf16"),
-    ([12000] * 3, 1, 64, 64, "bf16"), ([50] * 200, 1, 32, 64, "fp16"), ([70, 2500] * 40, 2, 64, 320, "bf16"), ([5, 100], 8, 7, 56, "fp16")])
+    ([300, 1000, 0, 700, 59], 60, 64, 64, "bf16"), ([2000, 33], 33, 128, 16, "fp16"), ([12000] * 3, 1, 64, 64, "bf16"), ([50] * 200, 1, 32, 64, "fp16"), ([70, 2500] * 40, 2, 64, 320, "bf16"), ([5, 100], 8, 7, 56, "fp16")])
 def test_attention_matches_the_formula(cuda_dev, lens, q_len, heads, page, dt):
     cache, table, lens = paged(cuda_dev, lens, page, DT[dt], len(lens) + heads)
     q = torch.randn(lens.numel() * q_len, heads, ROW, generator=gen(cuda_dev, 3), device=cuda_dev).to(DT[dt])
@@ -466,3 +466,75 @@ def test_shared_sequences_give_the_same_bits_every_time(cuda_dev, B, n, heads, q
     again = torch.empty_like(out)
     kernels.latent_attention(q, cache, table, lens, 0.07, again, workspace=ws)
     assert torch.equal(out, again)
+
+
+def test_without_programmatic_launches_the_results_are_the_same(cuda_dev):
+    from vic_b200 import kernels
+    from vic_b200.lib import lib
+    cache, table, lens = paged(cuda_dev, [3000, 65, 900], 64, torch.bfloat16, 41)
+    g = gen(cuda_dev, 42)
+    qin, w = torch.randn(3, 64, 192, generator=g, device=cuda_dev).to(torch.bfloat16), (torch.randn(64, 256, RANK, generator=g, device=cuda_dev) / 12).to(torch.bfloat16)
+    pos, f, kv = lens - 1, inv_freq(cuda_dev), torch.randn(3, ROW, generator=g, device=cuda_dev).to(torch.bfloat16)
+    slots = table.gather(1, (pos // 64).long()[:, None])[:, 0].long() * 64 + pos % 64
+    ws = torch.empty(kernels.latent_attention_workspace_bytes(), dtype=torch.uint8, device=cuda_dev)
+    start, got = cache.clone(), []
+    try:
+        for pdl in (1, 0):
+            lib().vib3_config_set(1, pdl)
+            cache.copy_(start)
+            q, o, y = (torch.empty(3, 64, n, dtype=torch.bfloat16, device=cuda_dev) for n in (ROW, RANK, 128))
+            kernels.latent_append(kv, None, 0.0, pos, slots, f, cache)
+            kernels.latent_query(qin, w[:, :128], pos, f, q)
+            kernels.latent_attention(q, cache, table, lens, 0.07, o, workspace=ws)
+            kernels.latent_value(o, w[:, 128:], y)
+            got.append((cache.clone(), q, o, y))
+    finally:
+        lib().vib3_config_set(1, 1)
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+def test_two_streams_with_workspaces_of_their_own(cuda_dev):
+    """Two attentions and the products of another step at the same time: nothing is shared but the cache that they read."""
+    from vic_b200 import kernels
+    cache, table, lens = paged(cuda_dev, [5000, 65, 900, 20000], 64, torch.bfloat16, 43)
+    q = torch.randn(4, 64, ROW, generator=gen(cuda_dev, 44), device=cuda_dev).to(torch.bfloat16)
+    want, _ = check_attention(q, cache, table, lens, 0.07)
+    w = (torch.randn(64, 128, RANK, generator=gen(cuda_dev, 45), device=cuda_dev) / 20).to(torch.bfloat16)
+    y0 = torch.empty(4, 64, 128, dtype=torch.bfloat16, device=cuda_dev)
+    kernels.latent_value(want, w, y0)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    ws = [torch.empty(kernels.latent_attention_workspace_bytes(), dtype=torch.uint8, device=cuda_dev) for _ in range(2)]
+    outs = [[torch.empty_like(want) for _ in range(20)] for _ in range(2)]
+    ys = [torch.empty_like(y0) for _ in range(20)]
+    for i in range(20):
+        for s in range(2):
+            with torch.cuda.stream(streams[s]):
+                kernels.latent_attention(q, cache, table, lens, 0.07, outs[s][i], workspace=ws[s])
+        with torch.cuda.stream(streams[2]):
+            kernels.latent_value(want, w, ys[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for s in outs for o in s) and all(torch.equal(y, y0) for y in ys)
+
+
+def test_operands_off_the_device_are_refused(cuda_dev):
+    from vic_b200 import kernels
+    cache, table, lens = paged(cuda_dev, [10], 8, torch.bfloat16, 46)
+    q, out = (torch.zeros(1, 4, n, dtype=torch.bfloat16, device=cuda_dev) for n in (ROW, RANK))
+    ws = torch.empty(kernels.latent_attention_workspace_bytes(), dtype=torch.uint8, device=cuda_dev)
+    with pytest.raises(ValueError):
+        kernels.latent_attention(q, cache, table.cpu(), lens, 0.1, out, workspace=ws)
+    with pytest.raises(ValueError):
+        kernels.latent_value(out, torch.zeros(4, 16, RANK, dtype=torch.bfloat16), torch.zeros(1, 4, 16, dtype=torch.bfloat16, device=cuda_dev))
+
+
+def test_nothing_beyond_the_workspace_and_the_table_is_touched(cuda_dev):
+    """Guard bytes on both sides of the workspace, guard entries around the table and the lengths."""
+    from vic_b200 import kernels
+    n = kernels.latent_attention_workspace_bytes()
+    big = torch.full((n + 512,), 0x5A, dtype=torch.uint8, device=cuda_dev)
+    cache, table, lens = paged(cuda_dev, [9000] * 40 + [0, 1], 64, torch.bfloat16, 47)
+    q = torch.randn(42, 64, ROW, generator=gen(cuda_dev, 48), device=cuda_dev).to(torch.bfloat16)
+    check_attention(q, cache, table, lens, 0.07, workspace=big[256:256 + n])
+    assert bool((big[:256] == 0x5A).all()) and bool((big[256 + n:] == 0x5A).all())

@@ -47,7 +47,7 @@ UNSUPPORTED, COUNT, NULL, ALIGN, SHAPE, CAPACITY = -1, -2, -3, -4, -5, -8
     *[(append, {n: 0}, NULL) for n in ("kv", "positions", "slots", "inv_freq", "cache")],
     (append, {"kv_dtype": 3}, UNSUPPORTED), (append, {"cache_dtype": F32}, UNSUPPORTED), (append, {"n_tokens": -1}, COUNT),
     (append, {"num_pages": 0}, COUNT), (append, {"page_size": 0}, COUNT), (append, {"row_stride": 568}, SHAPE),
-    (append, {"n_tokens": 2, "kv_stride": 568}, SHAPE), (append, {"kv": P + 2}, ALIGN), (append, {"kv_stride": 580}, ALIGN),
+    (append, {"n_tokens": 2, "kv_stride": 568}, SHAPE), (append, {"page_stride": 15 * 576}, SHAPE), (append, {"page_stride": 0}, SHAPE), (append, {"kv": P + 2}, ALIGN), (append, {"kv_stride": 580}, ALIGN),
     (append, {"kv_dtype": F32, "kv_stride": 578}, ALIGN), (append, {"row_stride": 580}, ALIGN), (append, {"cache": P + 8}, ALIGN),
     (append, {"page_stride": 16 * 576 + 4}, ALIGN), (append, {"norm": P + 2}, ALIGN),
     *[(query, {n: 0}, NULL) for n in ("q", "w", "positions", "inv_freq", "out")],

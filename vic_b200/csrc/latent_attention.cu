@@ -29,7 +29,7 @@ constexpr int kTileBytes = kChunks * kChunkBytes;
 constexpr int kQTmemChunks = 6, kSlots = 11, kTiles = 3, kSlotBytes = 2 * kChunkBytes;
 constexpr int kQOff = 0, kRingOff = (kChunks - kQTmemChunks) * kChunkBytes, kRopeOff = kRingOff + kSlots * kSlotBytes;
 constexpr int kMiscOff = kRopeOff + kTiles * kChunkBytes;
-constexpr int kAttThreads = 384;                          // copies, S, O, (none), eight warps for Q, the softmax and the results
+constexpr int kAttThreads = 384;                          // copies, S, O, (none: a warp reads its quarter of tensor memory), eight warps for Q, the softmax and the results
 constexpr int kSoftmaxThreads = 256;
 constexpr int kTmemCols = 512, kSCol = 256, kQCol = 320;  // O^T: 4 x 64 columns, S: 64, Q: 6 x 32
 static_assert(kQCol + 32 * kQTmemChunks <= kTmemCols, "tensor memory");
@@ -78,7 +78,7 @@ struct AttentionArgs {
 // is cut into equal shares whatever the lengths are; a sequence that a cut divides leaves parts that a second launch adds up.
 struct Plan {
     int begin, end;                        // this CTA's tiles on the line
-    int prefix, b, rb;                     // the first item: where it begins, sequence, row block
+    int prefix, b, rb, len, seen, tiles;   // the first item: where it begins, and what item_of says of it
     int share, shares, per, rem;           // share s begins at s * per + min(s, rem)
 };
 
@@ -90,7 +90,7 @@ struct Piece {
 
 // A row block costs what its tiles do and kPieceCost more (Q, the results, filling the pipe: 8000 to 10000 cycles), so on the line it begins
 // with a stretch without tiles.  (Without it a CTA with the ends of several short sequences took twice the average.)
-constexpr int kPieceCost = 3, kMinCost = 2;
+constexpr int kPieceCost = 4, kMinCost = 2;
 __device__ __forceinline__ int cost_of(const Piece& p) { return p.tiles ? p.tiles + kPieceCost : 0; }
 
 __device__ __forceinline__ int first_tile(const Plan& p, int share) { return share * p.per + min(share, p.rem); }
@@ -108,13 +108,19 @@ __device__ __forceinline__ void item_of(const AttentionArgs& a, int b, int rb, P
 struct Walk {
     const AttentionArgs& a;
     int b, rb, rb0, prefix, begin, end;
-    bool last;
+    bool last, known;
+    const Plan& plan;
     __device__ __forceinline__ Walk(const AttentionArgs& a_, const Plan& p, int rb_first)
-        : a(a_), b(p.b), rb(p.rb), rb0(rb_first), prefix(p.prefix), begin(p.begin), end(p.end), last(p.share == p.shares - 1) {}
+        : a(a_), b(p.b), rb(p.rb), rb0(rb_first), prefix(p.prefix), begin(p.begin), end(p.end), last(p.share == p.shares - 1), known(true), plan(p) {}
     __device__ __forceinline__ bool next(Piece& p, bool empty) {
 #pragma unroll 1
         while (b < a.batch && (prefix < end || last)) {
-            item_of(a, b, rb, p);
+            if (known) {
+                p.b = b; p.rb = rb; p.len = plan.len; p.seen = plan.seen; p.tiles = plan.tiles;
+                known = false;
+            } else {
+                item_of(a, b, rb, p);
+            }
             if (++rb == rb0 + a.blocks_per_lane) {
                 rb = rb0;
                 ++b;
@@ -209,7 +215,7 @@ __device__ __forceinline__ Plan make_plan(const AttentionArgs& a) {
     const int most = a.lanes == 1 ? gridDim.x : gridDim.x / a.lanes, items = a.batch * a.blocks_per_lane;
     const int run = (items + 31) >> 5, i0 = min(lane * run, items), i1 = min(i0 + run, items);
     const int b0 = a.blocks_per_lane == 1 ? i0 : i0 / a.blocks_per_lane, rb_first = row_lane * a.blocks_per_lane;
-    Piece p;
+    Piece p = {};
     int sum = 0;
     for (int i = i0, b = b0, x = i0 - b0 * a.blocks_per_lane; i < i1; ++i) {
         item_of(a, b, rb_first + x, p);
@@ -252,6 +258,9 @@ __device__ __forceinline__ Plan make_plan(const AttentionArgs& a) {
     plan.prefix = __shfl_sync(0xffffffffu, prefix, who);
     plan.b = hits ? __shfl_sync(0xffffffffu, b, who) : a.batch;      // nothing for a CTA beyond the shares
     plan.rb = __shfl_sync(0xffffffffu, rb_first + x, who);
+    plan.len = __shfl_sync(0xffffffffu, p.len, who);
+    plan.seen = __shfl_sync(0xffffffffu, p.seen, who);
+    plan.tiles = __shfl_sync(0xffffffffu, p.tiles, who);
     return plan;
 }
 
@@ -447,19 +456,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
             __syncwarp();
             bar_wait_warp(&sh.drain[1], 0);
         }
-    } else if (warp == 3) {
-        // ── Q of the later pieces into L2: fetched from HBM under the streaming tiles it took 5000 cycles between two pieces ──
-        for (bool first = true; ok && walk.next(p, false); first = false) {
-            if (first) continue;
-            for (int r = lane; r < a.block_rows; r += 32) {
-                const int row = p.rb * a.block_rows + r, j = a.by_heads(row);
-                if (row >= rows_all) break;
-                const T* q = (const T*)a.q + ((long long)p.b * a.q_len + j) * a.q_token + (row - j * a.heads) * a.q_head;
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + 64 * c));
-            }
-        }
-    } else {
+    } else if (warp >= 4) {
         // ── Q, softmax and results ──
         // Two teams of four warps, 32 keys each; warp w of a team has rows 16 w .. (their lanes in tensor memory), a thread two rows
         // and eight keys of each.  (A thread whose wait ran out goes on to the next common barrier, where all of them leave.)
@@ -767,6 +764,9 @@ __global__ void __launch_bounds__(kCombineThreads, 2) latent_combine_kernel(cons
     const int parts = own.z, c = own.w, team = parts <= kCombineAlone ? 1 : most;
     const int x = blockIdx.x * kCombineWarps + warp, mate = x & (team - 1), unit = x / team;
     if (parts < 2 || unit >= a.block_rows * kSplit) return;      // (the same for all warps of a block: team divides their number)
+    // (an entry that no CTA has written, after a wait that ran out, is whatever the workspace held)
+    if (c < 0 || parts > kMaxGrid || c + (parts - 1) * a.lanes >= kMaxGrid || own.x < 0 || own.x >= a.batch || own.y < 0 || own.y >= a.lanes * a.blocks_per_lane)
+        return;
     const int u = unit / kSplit;
     // rows r .. r + 3 of the block, values 128 g + 32 w + lane with g in [g0, g0 + GN)
     const int w = u & 3, r = (u >> 2) * 4, g0 = GN * (unit % kSplit), row0 = own.y * a.block_rows + r;
@@ -890,7 +890,10 @@ int launch_attention(const CUtensorMap& map, const AttentionArgs& a, int grid, c
     if (r) return r;
     const long long items = (long long)a.batch * a.lanes * a.blocks_per_lane;
     const int made = a.by_item ? (int)items : grid;
-    const int team = made <= 18 ? 8 : made <= 64 ? 4 : 2, split = made <= 4 ? 4 : 1;
+    // As many warps for a part's bytes as about two blocks per SM have: more blocks come in waves (four row blocks in 1024 blocks: 12 us
+    // instead of 5).
+    const int room = 2 * sm_count() + 24, units = a.block_rows / kCombineWarps * made;
+    const int split = units * 32 <= room ? 4 : 1, team = units * 8 <= room ? 8 : units * 4 <= room ? 4 : 2;
     const dim3 blocks((unsigned)(a.block_rows * team * split / kCombineWarps), (unsigned)made);
     return split == 4 ? launch_latent(latent_combine_kernel<T, 1>, blocks, kCombineThreads, 0, st, a, team)
                       : launch_latent(latent_combine_kernel<T, 4>, blocks, kCombineThreads, 0, st, a, team);

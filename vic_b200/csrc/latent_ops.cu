@@ -382,9 +382,11 @@ extern "C" int vib3_launch_latent_append_paged(const void* kv, int kv_dtype, lon
     if (!kv || !positions || !slots || !inv_freq || !cache) return VIB3_ERR_NULL;
     if (n_tokens < 0 || n_tokens > kLatentMaxTokens || num_pages <= 0 || page_size <= 0) return VIB3_ERR_COUNT;
     if (kv_dtype < L_F32 || kv_dtype > L_BF16 || (cache_dtype != L_F16 && cache_dtype != L_BF16)) return VIB3_ERR_UNSUPPORTED;
-    if (row_stride < kLatentRow || page_stride < 0 || (n_tokens > 1 && kv_stride < kLatentRow)) return VIB3_ERR_SHAPE;
     const int per16 = kv_dtype == L_F32 ? 4 : 8;
     if (off16(kv) || kv_stride % per16 || off16(norm_weight_or_null) || off16(cache) || page_stride % 8 || row_stride % 8) return VIB3_ERR_ALIGN;
+    if (row_stride < kLatentRow || page_stride < 0 || (num_pages > 1 && page_stride < row_stride * (page_size - 1) + kLatentRow) ||
+        (n_tokens > 1 && kv_stride < kLatentRow))
+        return VIB3_ERR_SHAPE;
     if (n_tokens == 0) return VIB3_OK;
     AppendArgs a{kv, kv_stride, norm_weight_or_null, eps, positions, slots, inv_freq, rope_scale, pairs, n_tokens, cache,
                  num_pages * page_size, page_size, page_stride, row_stride, status};
