@@ -760,9 +760,9 @@ __global__ void __launch_bounds__(kCombineThreads, 2) latent_combine_kernel(cons
     __shared__ float4 tops[2 * kCombineWarps];
     pdl_enter();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows_all = a.q_len * a.heads;
-    const int4 own = a.made_of[blockIdx.y];
+    const int4 own = a.made_of[blockIdx.x];      // (row blocks first: the blocks that return at once come last)
     const int parts = own.z, c = own.w, team = parts <= kCombineAlone ? 1 : most;
-    const int x = blockIdx.x * kCombineWarps + warp, mate = x & (team - 1), unit = x / team;
+    const int x = blockIdx.y * kCombineWarps + warp, mate = x & (team - 1), unit = x / team;
     if (parts < 2 || unit >= a.block_rows * kSplit) return;      // (the same for all warps of a block: team divides their number)
     // (an entry that no CTA has written, after a wait that ran out, is whatever the workspace held)
     if (c < 0 || parts > kMaxGrid || c + (parts - 1) * a.lanes >= kMaxGrid || own.x < 0 || own.x >= a.batch || own.y < 0 || own.y >= a.lanes * a.blocks_per_lane)
@@ -894,7 +894,7 @@ int launch_attention(const CUtensorMap& map, const AttentionArgs& a, int grid, c
     // instead of 5).
     const int room = 2 * sm_count() + 24, units = a.block_rows / kCombineWarps * made;
     const int split = units * 32 <= room ? 4 : 1, team = units * 8 <= room ? 8 : units * 4 <= room ? 4 : 2;
-    const dim3 blocks((unsigned)(a.block_rows * team * split / kCombineWarps), (unsigned)made);
+    const dim3 blocks((unsigned)made, (unsigned)(a.block_rows * team * split / kCombineWarps));
     return split == 4 ? launch_latent(latent_combine_kernel<T, 1>, blocks, kCombineThreads, 0, st, a, team)
                       : launch_latent(latent_combine_kernel<T, 4>, blocks, kCombineThreads, 0, st, a, team);
 }
