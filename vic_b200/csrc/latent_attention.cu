@@ -15,11 +15,11 @@
 // The tile of C that TMA brought once is operand of both products: K-major (its 576 values contiguous) in the first, and in the
 // second, through another descriptor of the same bytes, MN-major.  With the accumulator transposed its 256 columns fill all 128
 // lanes of tensor memory, so it stays there for the whole sequence, and the number of rows is the N of the MMA.
-// Per tile the pipe is busy 36 x 32 + 16 x 48 = 1920 cycles, HBM's share of an SM 3150.  What decides is how long a tile stays in
+// Per tile the pipe is busy 36 x 32 + 16 x 48 = 1920 cycles, HBM's share of an SM 3270 at 1.965 GHz.  What decides is how long a tile stays in
 // shared memory: load 2800 to 3500, S 1150, softmax 700, O 900 cycles.  With all of Q in shared memory there is room for two tiles
-// and a tile took 3500 cycles; with six of its nine chunks in tensor memory for two and three quarters, and it takes 2650 to 2750, HBM's rate.
-// Measured, 64 heads, bf16, with the adding launch: 128 sequences of 4100 tokens 124 us (5.0 TB/s; 138 to 144 us when the card
-// is held at its power limit), one of 131071 43 us, 32 of 1 to 16384 38 us, one of 4001 12.9 us.
+// and a tile took 3500 cycles; with six of its nine chunks in tensor memory for two and three quarters, and it takes 3200, HBM's rate.
+// Measured, 64 heads, bf16, with the adding launch: 128 sequences of 4100 tokens 125 us (5.0 TB/s; 144 us when the card
+// is held at its power limit), one of 131071 43 us, 32 of 1 to 16384 39 us, one of 4001 12.9 us.
 #include "latent_tc.cuh"
 
 namespace vib3 {

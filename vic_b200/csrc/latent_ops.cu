@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) latent_append_kernel(Append
 // with few instructions (warp-level MMAs fed by 16-byte copies spent their time on addresses: 500 queries of 64 heads in 32 us), and that
 // reads and writes overlap: a CTA per SM takes tile after tile, the ring (160 KB) runs ahead across them, and of two accumulators one is
 // stored while the other is filled.  (A CTA per tile, all of them loading and then all of them storing: 16.7 us; two CTAs per SM with a
-// third of the ring each, where a tile's loads waited for the tile before: 15.8; now 13.1 us, 4.4 TB/s.)  One query or value: 3.8 and 4.6 us.
+// third of the ring each, where a tile's loads waited for the tile before: 15.8; now 13.0 us, 4.4 TB/s.)  One query or value: 3.8 and 4.7 us.
 constexpr int kHeadTokens = 128, kHeadAChunk = kHeadTokens * 128, kHeadMaxStages = 12, kHeadMaxCols = 128;
 constexpr int kHeadOut = kHeadTokens * kHeadMaxCols * 2, kHeadRing = 160 * 1024;   // (two such tiles)
 constexpr int kHeadThreads = 320;          // copies, MMAs, four warps for the results, four for the rotation
