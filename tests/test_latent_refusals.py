@@ -71,6 +71,16 @@ def test_refusals(call, change, code):
     assert call(**change) == code
 
 
+@pytest.mark.parametrize("page_size,max_pages", [(16, (1 << 27) - 16), (8, (1 << 28) - 256), (1 << 20, 2047), (64, 0x7ffff000 // 64 + 1)])
+def test_lengths_whose_key_numbers_pass_32_bits_are_refused(page_size, max_pages):
+    # a table entry is looked up for 32 boxes of up to 64 keys at once: the last key number of that look is up to 2048 beyond the length
+    change = dict(page_size=page_size, page_stride=page_size * 576, max_pages=max_pages, table_stride=max_pages)
+    if (max_pages * page_size - 1) // 64 * 64 + 31 * 64 >= 1 << 31 or max_pages * page_size > 0x7ffff000:
+        assert attention(**change) == COUNT
+    else:
+        assert attention(**{**change, "workspace_bytes": 0}) == CAPACITY
+
+
 def test_a_call_without_tokens_launches_nothing():
     assert append(n_tokens=0) == 0 and query(n_tokens=0) == 0 and value(n_tokens=0) == 0
     assert attention(batch=0) == 0 and attention(q_len=0) == 0

@@ -918,8 +918,9 @@ extern "C" int vib3_launch_latent_attention_paged(const void* q, long long q_tok
     if (!q || !cache || !page_table || !seq_lens || !out || !workspace) return VIB3_ERR_NULL;
     if (dtype != L_F16 && dtype != L_BF16) return VIB3_ERR_UNSUPPORTED;
     if (page_size % 8) return VIB3_ERR_UNSUPPORTED;
+    // (the copying warp looks up table entries for 32 boxes at once, up to 2048 keys beyond the length, and key numbers have 32 bits)
     if (batch < 0 || q_len < 0 || heads <= 0 || heads > kLatentMaxHeads || num_pages <= 0 || num_pages > 0x7fffffff || page_size <= 0 ||
-        page_size > (1 << 20) || max_pages_per_seq <= 0 || (long long)max_pages_per_seq * page_size > 0x7fffff00 ||
+        page_size > (1 << 20) || max_pages_per_seq <= 0 || (long long)max_pages_per_seq * page_size > 0x7ffff000 ||
         (long long)batch * q_len > (1 << 20))
         return VIB3_ERR_COUNT;
     // (a tensor map's strides are below 2^40 bytes)
@@ -958,7 +959,7 @@ extern "C" int vib3_launch_latent_attention_paged(const void* q, long long q_tok
     a.lanes = blocks <= 8 ? blocks : 1;
     a.blocks_per_lane = blocks / a.lanes;
     // the kernel counts tiles (and what a row block costs beside them) in 32 bits
-    if ((long long)batch * a.blocks_per_lane * (most_tiles + kPieceCost) > 0x7fffffff) return VIB3_ERR_COUNT;
+    if ((long long)batch * a.blocks_per_lane * (most_tiles + kPieceCost) > 0x7fffff00) return VIB3_ERR_COUNT;
     a.by_item = (long long)batch * blocks <= kMaxGrid;
     a.min_cost = kMinCost;
     const int grid = sms / a.lanes * a.lanes;
