@@ -370,7 +370,9 @@ int vib3_launch_moe_grouped_int4(void* handle, const void* x, int x_dtype, int x
  * matrix is contiguous; dtypes are VIB3_X_F16 or VIB3_X_BF16, one for all 16-bit operands of a call.  n_tokens, batch or q_len 0:
  * nothing is launched.  The launches are programmatic dependents that read nothing before their predecessor has finished.
  * inv_freq: 32 doubles on the device, one per pair of position values; the angle position * inv_freq[i] is formed in 64 bits.
- * pairs != 0: value 2 i turns with value 2 i + 1; 0: value i with value i + 32.  rope_scale multiplies the rotated values. */
+ * pairs != 0: value 2 i turns with value 2 i + 1; 0: value i with value i + 32.  rope_scale multiplies the rotated values.
+ * status (may be NULL): one int on the device that a launch sets bits of; VIB3_STATUS_TIMEOUT, from every launch but the append, means
+ * that a wait inside the kernel gave up and the results are not valid. */
 
 /* Append n_tokens rows to the cache: kv [n_tokens][576] (VIB3_X_*, kv_stride apart) holds the latents and the unrotated
  * position values.  latent = kv[:512] / sqrt(mean of squares + eps) * norm_weight (norm_weight: 512 values of the cache's type;
@@ -388,12 +390,12 @@ int vib3_launch_latent_append_paged(const void* kv, int kv_dtype, long long kv_s
 int vib3_launch_latent_query(const void* q, long long q_token_stride, long long q_head_stride, const void* w_uk, long long w_head_stride,
                              const int* positions, const double* inv_freq, float rope_scale, int pairs, void* out,
                              long long out_token_stride, long long out_head_stride, int n_tokens, int heads, int nope, int dtype,
-                             void* stream);
+                             int* status, void* stream);
 /* The heads' outputs: o [n_tokens][heads][512], w_uv [heads][value][512]: out[t][h][v] = o[t][h] . w_uv[h][v].  value: a multiple
  * of 16 up to 256.  (w_uk and w_uv may be views of one matrix [heads][nope + value][512].) */
 int vib3_launch_latent_value(const void* o, long long o_token_stride, long long o_head_stride, const void* w_uv, long long w_head_stride,
                              void* out, long long out_token_stride, long long out_head_stride, int n_tokens, int heads, int value,
-                             int dtype, void* stream);
+                             int dtype, int* status, void* stream);
 /* Attention of the q_len newest tokens of each of `batch` sequences over the paged cache, in the latent space.  q [batch *
  * q_len][heads][576] (sequence b's tokens at rows b * q_len ..), seq_lens[b]: keys of sequence b with its new tokens; token j of
  * q_len stands at position seq_lens[b] - q_len + j and sees the keys up to that position (none, if it is negative: out = 0, lse =

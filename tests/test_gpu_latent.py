@@ -408,6 +408,19 @@ def test_products_of_broadcast_and_overlapping_operands(cuda_dev, which):
     assert_rounded(out[..., RANK:], rotate64(q[..., n:], pos, f, True), 16 * 2.0 ** -24 * 2 * q[..., n:].double().abs().amax(-1, keepdim=True))
 
 
+def test_products_leave_the_status_as_it_was(cuda_dev):
+    from vic_b200 import kernels as K
+    status = torch.tensor([1 << 20], dtype=torch.int32, device=cuda_dev)
+    for tokens in (1, 300):
+        q, w = (torch.ones(*s, dtype=torch.bfloat16, device=cuda_dev) for s in ((tokens, 8, 192), (8, 256, 512)))
+        lat, out = torch.zeros(tokens, 8, 576, dtype=q.dtype, device=cuda_dev), torch.zeros(tokens, 8, 128, dtype=q.dtype, device=cuda_dev)
+        K.latent_query(q, w[:, :128], torch.zeros(tokens, dtype=torch.int32, device=cuda_dev), torch.ones(32, dtype=torch.float64, device=cuda_dev),
+                       lat, status=status)
+        K.latent_value(lat[:, :, :512], w[:, 128:], out, status=status)
+        assert lat[:, :, :512].unique().tolist() == [128.0] and out.unique().tolist() == [65536.0]
+    assert status.tolist() == [1 << 20]
+
+
 @pytest.mark.parametrize("tokens", [127, 128, 129, 256, 257])
 @pytest.mark.parametrize("heads", [1, 8, 64])
 def test_products_at_the_borders_of_their_tiles(cuda_dev, tokens, heads):

@@ -20,14 +20,14 @@ def append(**k):
 
 def query(**k):
     a = dict(q=P, q_token=2 * 192, q_head=192, w=P, w_head=128 * 512, positions=P, inv_freq=P, rope_scale=1.0, pairs=1, out=P,
-             out_token=2 * 576, out_head=576, n_tokens=2, heads=2, nope=128, dtype=BF16, stream=0)
+             out_token=2 * 576, out_head=576, n_tokens=2, heads=2, nope=128, dtype=BF16, status=0, stream=0)
     a.update(k)
     return lib().vib3_launch_latent_query(*a.values())
 
 
 def value(**k):
     a = dict(o=P, o_token=1024, o_head=512, w=P, w_head=128 * 512, out=P, out_token=256, out_head=128, n_tokens=2, heads=2, value=128,
-             dtype=F16, stream=0)
+             dtype=F16, status=0, stream=0)
     a.update(k)
     return lib().vib3_launch_latent_value(*a.values())
 

@@ -105,9 +105,9 @@ class LatentAttention:
         torch.matmul(x, self.w_kv.t(), out=self.kv_in[:T])
         torch.matmul(x, self.w_q.t(), out=self.q_in[:T])
         kernels.latent_append(self.kv_in[:T], self.kv_norm, sh.eps, pos, cache.slots[:T], self.inv_freq, rows, status=self.status)
-        kernels.latent_query(self.q_in[:T].view(T, sh.heads, sh.nope + LATENT_ROPE), self.kv_b[:, :sh.nope], pos, self.inv_freq, self.q[:T])
+        kernels.latent_query(self.q_in[:T].view(T, sh.heads, sh.nope + LATENT_ROPE), self.kv_b[:, :sh.nope], pos, self.inv_freq, self.q[:T], status=self.status)
         kernels.latent_attention(self.q[:T], rows, cache.table, cache.lens, sh.scale, self.o[:T], workspace=self.workspace, status=self.status)
-        kernels.latent_value(self.o[:T], self.kv_b[:, sh.nope:], self.v[:T])
+        kernels.latent_value(self.o[:T], self.kv_b[:, sh.nope:], self.v[:T], status=self.status)
         torch.matmul(self.v[:T].view(T, sh.heads * sh.value), self.w_o.t(), out=self.out[:T])
         return self.out[:T]
 

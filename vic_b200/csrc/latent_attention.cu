@@ -728,7 +728,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
         }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (!ok && lane == 0 && a.status) atomicOr(a.status, 4 /* VIB3_STATUS_TIMEOUT */);
+    if (!ok && lane == 0 && a.status) atomicOr(a.status, kStatusTimeout);
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {

@@ -21,6 +21,7 @@ constexpr int kRope = 64;             // position values of a row
 constexpr int kLatentRow = kRank + kRope;
 constexpr int kLatentMaxHeads = 128;
 constexpr int kStatusBadPage = 1;     // VIB3_STATUS_MISSING_PAGE
+constexpr int kStatusTimeout = 4;     // VIB3_STATUS_TIMEOUT
 
 // The activation codes of the C ABI.
 enum LatentDType : int { L_F32 = 0, L_F16 = 1, L_BF16 = 2 };

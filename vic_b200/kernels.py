@@ -375,9 +375,10 @@ def latent_append(kv: torch.Tensor, norm_weight: Optional[torch.Tensor], eps: fl
 
 
 def latent_query(q: torch.Tensor, w_uk: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, out: torch.Tensor,
-                 pairs: bool = True, rope_scale: float = 1.0, stream: Optional[int] = None) -> None:
+                 pairs: bool = True, rope_scale: float = 1.0, status: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> None:
     """The heads' queries in the latent space (cuda/src/kernels.cu:1679 for T tokens): q [T, H, nope + 64], w_uk [H, nope, 512] ->
-    out [T, H, 576] = (q[..., :nope] . w_uk, q[..., nope:] rotated).  One 16-bit dtype; w_uk may be a view of [H, nope + value, 512]."""
+    out [T, H, 576] = (q[..., :nope] . w_uk, q[..., nope:] rotated).  One 16-bit dtype; w_uk may be a view of [H, nope + value, 512].
+    ``status`` [1] int32 receives VIB3_STATUS_TIMEOUT."""
     (T, H, width), (q0, q1, q2) = q.shape, q.stride()
     (heads, nope, R), (w0, w1, w2) = w_uk.shape, w_uk.stride()
     o0, o1, o2 = out.stride()
@@ -396,18 +397,20 @@ def latent_query(q: torch.Tensor, w_uk: torch.Tensor, positions: torch.Tensor, i
         raise ValueError("one dtype, fp16 or bf16, expected")
     launch = (_latent or _bind_latent())[1]
     dev = _current_device()     # (a launch on another one would read through a foreign context)
-    if not (dev == q.get_device() == w_uk.get_device() == positions.get_device() == inv_freq.get_device() == out.get_device()):
-        raise _foreign(q, w_uk, positions, inv_freq, out)
+    if not (dev == q.get_device() == w_uk.get_device() == positions.get_device() == inv_freq.get_device() == out.get_device()
+            == (q if status is None else status).get_device()):
+        raise _foreign(q, w_uk, positions, inv_freq, out, status)
     err = launch(
         q.data_ptr(), q0, q1, w_uk.data_ptr(), w0, positions.data_ptr(), inv_freq.data_ptr(), rope_scale, 1 if pairs else 0, out.data_ptr(),
-        o0, o1, T, H, nope, _X_CODES[dt], _current_stream(dev) if stream is None else stream)
+        o0, o1, T, H, nope, _X_CODES[dt], 0 if status is None else status.data_ptr(), _current_stream(dev) if stream is None else stream)
     if err:
         check("latent_query", err)
 
 
-def latent_value(o: torch.Tensor, w_uv: torch.Tensor, out: torch.Tensor, stream: Optional[int] = None) -> None:
+def latent_value(o: torch.Tensor, w_uv: torch.Tensor, out: torch.Tensor, status: Optional[torch.Tensor] = None,
+                 stream: Optional[int] = None) -> None:
     """The heads' outputs from their weighted latents (cuda/src/kernels.cu:1624 for T tokens): o [T, H, 512], w_uv [H, value, 512] ->
-    out [T, H, value].  One 16-bit dtype."""
+    out [T, H, value].  One 16-bit dtype.  ``status`` [1] int32 receives VIB3_STATUS_TIMEOUT."""
     (T, H, width), (i0, i1, i2) = o.shape, o.stride()
     (heads, value, R), (w0, w1, w2) = w_uv.shape, w_uv.stride()
     o0, o1, o2 = out.stride()
@@ -422,10 +425,10 @@ def latent_value(o: torch.Tensor, w_uv: torch.Tensor, out: torch.Tensor, stream:
         raise ValueError("one dtype, fp16 or bf16, expected")
     launch = (_latent or _bind_latent())[2]
     dev = _current_device()     # (a launch on another one would read through a foreign context)
-    if not (dev == o.get_device() == w_uv.get_device() == out.get_device()):
-        raise _foreign(o, w_uv, out)
+    if not (dev == o.get_device() == w_uv.get_device() == out.get_device() == (o if status is None else status).get_device()):
+        raise _foreign(o, w_uv, out, status)
     err = launch(o.data_ptr(), i0, i1, w_uv.data_ptr(), w0, out.data_ptr(), o0, o1, T, H, value, _X_CODES[dt],
-                                         _current_stream(dev) if stream is None else stream)
+                 0 if status is None else status.data_ptr(), _current_stream(dev) if stream is None else stream)
     if err:
         check("latent_value", err)
 

@@ -91,8 +91,8 @@ SIGNATURES = {
     "vib3_launch_rms_norm_f32": (_i, [_vp, _vp, _vp, _i, _f, _vp]),
     "vib3_launch_residual_rms_norm": (_i, [_vp, _i, _vp, _i, _i, _vp, _i, _vp, _f, _i, _vp, _i, _i, _i, _i, _vp]),
     "vib3_launch_latent_append_paged": (_i, [_vp, _i, _ll, _vp, _f, _vp, _vp, _vp, _f, _i, _i, _vp, _i, _ll, _i, _ll, _ll, _vp, _vp]),
-    "vib3_launch_latent_query": (_i, [_vp, _ll, _ll, _vp, _ll, _vp, _vp, _f, _i, _vp, _ll, _ll, _i, _i, _i, _i, _vp]),
-    "vib3_launch_latent_value": (_i, [_vp, _ll, _ll, _vp, _ll, _vp, _ll, _ll, _i, _i, _i, _i, _vp]),
+    "vib3_launch_latent_query": (_i, [_vp, _ll, _ll, _vp, _ll, _vp, _vp, _f, _i, _vp, _ll, _ll, _i, _i, _i, _i, _vp, _vp]),
+    "vib3_launch_latent_value": (_i, [_vp, _ll, _ll, _vp, _ll, _vp, _ll, _ll, _i, _i, _i, _i, _vp, _vp]),
     "vib3_latent_attention_workspace_bytes": (C.c_size_t, []),
     "vib3_launch_latent_attention_paged": (_i, [_vp, _ll, _ll, _vp, _ll, _i, _ll, _ll, _vp, _i, _i, _vp, _i, _i, _i, _f, _i, _vp, _ll,
                                                 _ll, _vp, _vp, C.c_size_t, _vp, _vp]),
