@@ -67,6 +67,25 @@ def test_a_sequence_has_no_more_pages_than_its_table():
     assert c.lens.tolist() == [1, 0, 0]
 
 
+def test_a_layer_takes_the_rows_of_the_step_and_no_others():
+    from vic_b200.attention import LatentAttention
+    from vic_b200.core_types import LatentShape
+    c = make(max_tokens=12)
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    sh = LatentShape("small", 64, 2, 16, 16, 10000.0, 1e-6)
+    layer = LatentAttention(sh, z(2 * 80, 64), z(576, 64), z(512), z(2, 32, 512), z(64, 32), max_tokens=12, workspace=torch.zeros(16, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="rows"):
+        layer.forward(z(3, 64), c, 0)                           # no step yet
+    c.begin_step([4, 4, 4])
+    c.begin_step([1, 1, 1])
+    for rows in (6, 12):                                        # the slots behind row 3 are the older step's
+        with pytest.raises(ValueError, match="rows"):
+            layer.forward(z(rows, 64), c, 0)
+    with pytest.raises(Exception):
+        c.begin_step([30, 0, 0])                                # refused: the step stays the one before
+    assert c.step_rows == 3
+
+
 def test_bad_layouts_are_refused():
     with pytest.raises(ValueError):
         make(page_size=12)

@@ -34,6 +34,7 @@ class LatentCache:
         self.positions = torch.zeros(max_tokens, dtype=torch.int32, device=device)
         self.slots = torch.full((max_tokens,), -1, dtype=torch.int64, device=device)
         self.host_lens: List[int] = [0] * max_sequences
+        self.step_rows = 0      # rows of the step that the buffers describe
         self._pages_of: List[List[int]] = [[] for _ in range(max_sequences)]
         self._free = list(range(pages - 1, -1, -1))
 
@@ -58,7 +59,7 @@ class LatentCache:
             slots += [-1] * pad + [own[p // self.page_size] * self.page_size + p % self.page_size for p in range(first, first + k)]
             self.host_lens[b] = first + k
         table = [own + [0] * (self.max_pages - len(own)) for own in self._pages_of]
-        n = len(positions)
+        n = self.step_rows = len(positions)
         self.positions[:n].copy_(torch.tensor(positions, dtype=torch.int32))
         self.slots[:n].copy_(torch.tensor(slots, dtype=torch.int64))
         self.table.copy_(torch.tensor(table, dtype=torch.int32))
@@ -99,8 +100,8 @@ class LatentAttention:
     def forward(self, x: torch.Tensor, cache: LatentCache, layer: int) -> torch.Tensor:
         """The step that ``cache.begin_step`` laid out.  Returns a view of ``self.out``."""
         sh, T = self.shape, x.shape[0]
-        if T > self.max_tokens or T % cache.max_sequences:
-            raise ValueError("x: a row for each of the step's sequences * q_len tokens expected")
+        if T > self.max_tokens or T != cache.step_rows:      # (the slots behind the step's rows are an older step's)
+            raise ValueError(f"x: the step's {cache.step_rows} rows (sequences * q_len) expected, at most {self.max_tokens}; got {T}")
         rows, pos = cache.rows[layer], cache.positions[:T]
         torch.matmul(x, self.w_kv.t(), out=self.kv_in[:T])
         torch.matmul(x, self.w_q.t(), out=self.q_in[:T])
