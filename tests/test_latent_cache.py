@@ -67,6 +67,20 @@ def test_a_sequence_has_no_more_pages_than_its_table():
     assert c.lens.tolist() == [1, 0, 0]
 
 
+def test_the_table_follows_pages_that_come_and_go():
+    c = make(pages=12)
+    steps = [[9, 8, 1], [0, 1, 0], "release 1", [8, 3, 0], "release 0", "release 2", [1, 0, 20], [0, 0, 0], [7, 1, 1], [1, 0, 0]]
+    for s in steps:
+        if isinstance(s, str):
+            c.release(int(s[-1]))
+            continue
+        c.begin_step(s)
+        used = [p for own in c._pages_of for p in own]
+        assert len(used) == len(set(used)) and not set(used) & set(c._free) and len(used) + len(c._free) == 12
+        for b, own in enumerate(c._pages_of):
+            assert len(own) == -(-c.host_lens[b] // 8) and c.table[b].tolist() == own + [0] * (4 - len(own))
+
+
 def test_a_layer_takes_the_rows_of_the_step_and_no_others():
     from vic_b200.attention import LatentAttention
     from vic_b200.core_types import LatentShape

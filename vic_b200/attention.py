@@ -30,6 +30,8 @@ class LatentCache:
         self.page_size, self.max_sequences, self.max_pages, self.max_tokens = page_size, max_sequences, max_pages, max_tokens
         self.rows = torch.zeros(layers, pages, page_size, LATENT_ROW, dtype=dtype, device=device)
         self.table = torch.zeros(max_sequences, max_pages, dtype=torch.int32, device=device)
+        self._host_table = torch.zeros(max_sequences, max_pages, dtype=torch.int32)     # (only new pages change it: most steps bring none)
+        self._table_changed = False
         self.lens = torch.zeros(max_sequences, dtype=torch.int32, device=device)
         self.positions = torch.zeros(max_tokens, dtype=torch.int32, device=device)
         self.slots = torch.full((max_tokens,), -1, dtype=torch.int64, device=device)
@@ -54,20 +56,25 @@ class LatentCache:
             own, first = self._pages_of[b], self.host_lens[b]
             while len(own) < need[b]:
                 own.append(self._free.pop())
+                self._host_table[b, len(own) - 1] = own[-1]
+                self._table_changed = True
             pad = q_len - k
             positions += [0] * pad + list(range(first, first + k))
             slots += [-1] * pad + [own[p // self.page_size] * self.page_size + p % self.page_size for p in range(first, first + k)]
             self.host_lens[b] = first + k
-        table = [own + [0] * (self.max_pages - len(own)) for own in self._pages_of]
         n = self.step_rows = len(positions)
         self.positions[:n].copy_(torch.tensor(positions, dtype=torch.int32))
         self.slots[:n].copy_(torch.tensor(slots, dtype=torch.int64))
-        self.table.copy_(torch.tensor(table, dtype=torch.int32))
+        if self._table_changed:
+            self.table.copy_(self._host_table)      # (from pageable memory: read before the call returns)
+            self._table_changed = False
         self.lens.copy_(torch.tensor(self.host_lens, dtype=torch.int32))
 
     def release(self, sequence: int) -> None:
         """Forget a sequence; its pages may go to others."""
         self._free += self._pages_of[sequence][::-1]
+        self._host_table[sequence] = 0
+        self._table_changed = True
         self._pages_of[sequence] = []
         self.host_lens[sequence] = 0
 
