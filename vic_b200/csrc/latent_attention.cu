@@ -953,7 +953,7 @@ extern "C" int vib3_launch_latent_attention_paged(const void* q, long long q_tok
     const int sms = sm_count() < kMaxGrid ? sm_count() : kMaxGrid;
     const long long rows = (long long)q_len * heads, most_tiles = ((long long)max_pages_per_seq * page_size + kTileKeys - 1) / kTileKeys;
     // Half row blocks where the whole ones would leave half of the SMs without work: the cache is then read twice (from L2), the
-    // results of a CTA, 128 KB at 30 bytes per cycle, are halved.
+    // results of a CTA, 128 KB at 27 bytes per cycle, are halved.
     a.block_rows = rows <= 32 || (rows + kTileRows - 1) / kTileRows * batch * most_tiles <= sms ? kTileRows / 2 : kTileRows;
     const int blocks = (int)((rows + a.block_rows - 1) / a.block_rows);
     a.lanes = blocks <= 8 ? blocks : 1;
