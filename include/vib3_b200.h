@@ -317,7 +317,8 @@ int vib3_launch_moe_layer_int4_paged_noalloc(const void* x, int x_dtype, const v
  * (cuda/src/kernels.cu:1132, called at src/runtime/engine.rs:5302) and the next rms_norm_f32 (:1178, called at
  * engine.rs:5072) — as one launch over n_tokens rows: hidden[t] += delta[t] + delta2[t] (either may be NULL;
  * delta2 is fp32 with a stride in floats: e.g. the previous MoE sublayer's output summed over expert-parallel ranks),
- * x_out[t] = cast(hidden[t] * inv_rms(hidden[t]) * weight) (weight_f16 NULL: no weight).  Dtypes VIB3_X_*;
+ * x_out[t] = cast(hidden[t] * inv_rms(hidden[t]) * weight) (weight fp16, or bf16 with bit 2 of `center` (value 4);
+ * NULL: no weight).  Dtypes VIB3_X_*;
  * strides of delta and x_out in bytes, of hidden in floats.  center != 0 (no counterpart in the reference) removes
  * the row's mean before normalising: for stacks of synthetic layers whose uniformly drawn INT4 codes have mean -0.5
  * (a common term that feeds itself through the residual stream).  Bit 1 of `center` (value 2): the launch is a
@@ -328,7 +329,7 @@ int vib3_launch_moe_layer_int4_paged_noalloc(const void* x, int x_dtype, const v
  * launch that follows, a layer is this launch plus the MoE launches. */
 int vib3_launch_residual_rms_norm(float* hidden, int hidden_stride, const void* delta_or_null, int delta_dtype,
                                   int delta_stride_bytes, const float* delta2_or_null, int delta2_stride,
-                                  const void* weight_f16_or_null, float eps, int center, void* x_out, int x_dtype,
+                                  const void* weight_or_null, float eps, int center, void* x_out, int x_dtype,
                                   int x_stride_bytes, int hidden_dim, int n_tokens, void* stream);
 
 /* ── Grouped multi-token layer (every distinct expert read once; tcgen05 tensor-core tiles) ── */

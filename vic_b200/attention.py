@@ -121,7 +121,8 @@ class LatentAttention:
 
 
 class DecodeLayer:
-    """h += attention(norm(h)), h += moe(norm(h)) for a step's rows: ``moe`` is a MoeDecoder (one row) or a GroupedDecoder."""
+    """h += attention(norm(h)), h += moe(norm(h)) for a step's rows: ``moe`` is a MoeDecoder (one row) or a GroupedDecoder.
+    The norms' weights [hidden] are fp16 or bf16."""
 
     def __init__(self, attention: LatentAttention, moe, layer: int, attention_norm: torch.Tensor, moe_norm: torch.Tensor, eps: float = 1e-6):
         self.attention, self.moe, self.layer = attention, moe, layer

@@ -280,6 +280,18 @@ __device__ __forceinline__ float block_inv_rms(float ss, int H, float eps, float
     return 1.0f / rms;
 }
 
+// Four norm weights of a 16-bit type from two words, and one of them.
+__device__ __forceinline__ float4 weights4(uint2 v, __half) {
+    const __half2 a = *reinterpret_cast<const __half2*>(&v.x), b = *reinterpret_cast<const __half2*>(&v.y);
+    return make_float4(__low2float(a), __high2float(a), __low2float(b), __high2float(b));
+}
+__device__ __forceinline__ float4 weights4(uint2 v, __nv_bfloat16) {
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xFFFF0000u), __uint_as_float(v.y << 16),
+                       __uint_as_float(v.y & 0xFFFF0000u));
+}
+__device__ __forceinline__ float weight1(__half v) { return __half2float(v); }
+__device__ __forceinline__ float weight1(__nv_bfloat16 v) { return __bfloat162float(v); }
+
 __device__ __forceinline__ void store_x(void* out, int dtype, int d, float v) {
     if (dtype == X_F32) reinterpret_cast<float*>(out)[d] = v;
     else if (dtype == X_F16) reinterpret_cast<__half*>(out)[d] = __float2half_rn(v);
@@ -290,11 +302,11 @@ __device__ __forceinline__ void store_x(void* out, int dtype, int d, float v) {
 // VEC (1024 threads): H a multiple of 4 and at most 8192, 16-byte aligned rows: a thread keeps its (at most two)
 // 4-column items in registers — every load is requested before anything is stored, one pass over the row.  Two items
 // per thread rather than eight in a quarter of the threads: the kernel runs once per layer on cold instruction caches,
-// and its time is the code it has to fetch.  Otherwise 256 threads and three passes.
-template <bool VEC>
+// and its time is the code it has to fetch.  Otherwise 256 threads and three passes.  TW: the weights' type, a kernel each for the same reason.
+template <bool VEC, typename TW>
 __global__ void __launch_bounds__(VEC ? 1024 : 256) residual_rms_norm_kernel(float* __restrict__ hidden, int hidden_stride, const void* __restrict__ delta,
                                                                 int delta_dtype, int delta_stride, const float* __restrict__ delta2,
-                                                                int delta2_stride, const __half* __restrict__ weight, float eps,
+                                                                int delta2_stride, const TW* __restrict__ weight, float eps,
                                                                 int flags, void* __restrict__ x_out, int x_dtype, int x_stride, int H) {
     __shared__ float red[256];
     const int t = blockIdx.x, tid = threadIdx.x;
@@ -315,7 +327,7 @@ __global__ void __launch_bounds__(VEC ? 1024 : 256) residual_rms_norm_kernel(flo
 #pragma unroll
         for (int i = 0; i < kItems; ++i) {
             const int it = tid + kThreads * i;
-            wv[i] = make_uint2(0x3C003C00u, 0x3C003C00u);   // 1.0
+            wv[i] = make_uint2(0u, 0u);
             if (it < n4 && weight) wv[i] = reinterpret_cast<const uint2*>(weight)[it];
         }
         asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -372,10 +384,10 @@ __global__ void __launch_bounds__(VEC ? 1024 : 256) residual_rms_norm_kernel(flo
             const int it = tid + kThreads * i;
             if (it < n4) {
                 if (drow || d2row) reinterpret_cast<float4*>(row)[it] = h[i];
-                const __half2 w0 = *reinterpret_cast<const __half2*>(&wv[i].x), w1 = *reinterpret_cast<const __half2*>(&wv[i].y);
+                const float4 w = weights4(wv[i], TW());
                 float v[4] = {(h[i].x - mean) * inv_rms, (h[i].y - mean) * inv_rms, (h[i].z - mean) * inv_rms, (h[i].w - mean) * inv_rms};
                 if (weight) {
-                    v[0] *= __low2float(w0); v[1] *= __high2float(w0); v[2] *= __low2float(w1); v[3] *= __high2float(w1);
+                    v[0] *= w.x; v[1] *= w.y; v[2] *= w.z; v[3] *= w.w;
                 }
 #pragma unroll
                 for (int c = 0; c < 4; ++c) store_x(xrow, x_dtype, 4 * it + c, v[c]);
@@ -397,13 +409,14 @@ __global__ void __launch_bounds__(VEC ? 1024 : 256) residual_rms_norm_kernel(flo
         const float inv_rms = block_inv_rms(ss, H, eps, red);
         for (int d = tid; d < H; d += 256) {
             float v = (row[d] - mean) * inv_rms;
-            if (weight) v *= __half2float(weight[d]);
+            if (weight) v *= weight1(weight[d]);
             store_x(xrow, x_dtype, d, v);
         }
     }
 }
 
-static int launch_norm(float* hidden, int hidden_stride, const void* delta, int delta_dtype, int delta_stride, const float* delta2,
+template <typename TW>
+int launch_norm_of(float* hidden, int hidden_stride, const void* delta, int delta_dtype, int delta_stride, const float* delta2,
                        int delta2_stride, const void* weight, float eps, int center, void* x_out, int x_dtype, int x_stride, int H,
                        int n_tokens, cudaStream_t st) {
     const bool vec = H % 4 == 0 && H <= 8192 && ((uintptr_t)hidden & 15) == 0 && (hidden_stride & 3) == 0 && ((uintptr_t)delta & 15) == 0 &&
@@ -415,12 +428,21 @@ static int launch_norm(float* hidden, int hidden_stride, const void* delta, int 
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = g_use_pdl.load(std::memory_order_relaxed) ? 1 : 0;
     cfg.attrs = attr; cfg.numAttrs = 1;
-    const __half* w16 = (const __half*)weight;
+    const TW* w16 = (const TW*)weight;
     if (vec)
-        return (int)cudaLaunchKernelEx(&cfg, residual_rms_norm_kernel<true>, hidden, hidden_stride, delta, delta_dtype, delta_stride, delta2,
+        return (int)cudaLaunchKernelEx(&cfg, residual_rms_norm_kernel<true, TW>, hidden, hidden_stride, delta, delta_dtype, delta_stride, delta2,
                                        delta2_stride, w16, eps, center, x_out, x_dtype, x_stride, H);
-    return (int)cudaLaunchKernelEx(&cfg, residual_rms_norm_kernel<false>, hidden, hidden_stride, delta, delta_dtype, delta_stride, delta2,
+    return (int)cudaLaunchKernelEx(&cfg, residual_rms_norm_kernel<false, TW>, hidden, hidden_stride, delta, delta_dtype, delta_stride, delta2,
                                    delta2_stride, w16, eps, center, x_out, x_dtype, x_stride, H);
+}
+
+// Bit 2 of `flags`: the weights are bf16.
+static int launch_norm(float* hidden, int hidden_stride, const void* delta, int delta_dtype, int delta_stride, const float* delta2,
+                       int delta2_stride, const void* weight, float eps, int flags, void* x_out, int x_dtype, int x_stride, int H,
+                       int n_tokens, cudaStream_t st) {
+    const auto launch = flags & 4 ? launch_norm_of<__nv_bfloat16> : launch_norm_of<__half>;
+    return launch(hidden, hidden_stride, delta, delta_dtype, delta_stride, delta2, delta2_stride, weight, eps, flags, x_out, x_dtype, x_stride, H,
+                  n_tokens, st);
 }
 
 // Reference signature (cuda/src/kernels.cu:1178): fp32 in, fp32 out, fp16 weight, one vector.
@@ -440,7 +462,7 @@ extern "C" int vib3_launch_rms_norm_f32(const void* input, void* output, const v
 // rms_norm_f32 of the next sublayer: src/runtime/engine.rs:5302, :5072) as ONE launch for n_tokens rows:
 //   hidden[t] += delta[t] + delta2[t]   (delta: the other sublayer's output, fp32 / fp16 / bf16, or NULL; delta2: fp32 or
 //                                        NULL, e.g. the sum over expert-parallel ranks of the previous MoE sublayer's outputs)
-//   x_out[t]   = cast(hidden[t] * inv_rms(hidden[t]) * weight)      (weight fp16 or NULL; x_out fp32 / fp16 / bf16)
+//   x_out[t]   = cast(hidden[t] * inv_rms(hidden[t]) * weight)      (weight fp16, with bit 2 of center bf16, or NULL; x_out fp32 / fp16 / bf16)
 // center != 0 (not in the reference): the row's mean is removed first, x = (hidden - mean) * inv_rms(hidden - mean) * weight.
 // For stacks of SYNTHETIC layers: INT4 codes drawn uniformly from [-8, 7] have mean -0.5, so every output row of such a
 // matrix carries a common term proportional to the sum of its input; through a residual stream that term feeds itself and
@@ -449,13 +471,13 @@ extern "C" int vib3_launch_rms_norm_f32(const void* input, void* output, const v
 // launch plus the MoE launches.
 extern "C" int vib3_launch_residual_rms_norm(float* hidden, int hidden_stride, const void* delta, int delta_dtype,
                                              int delta_stride_bytes, const float* delta2, int delta2_stride,
-                                             const void* weight_f16, float eps, int center, void* x_out, int x_dtype,
+                                             const void* weight_or_null, float eps, int center, void* x_out, int x_dtype,
                                              int x_stride_bytes, int hidden_dim, int n_tokens, void* stream) {
     if (!hidden || !x_out) return VIB3_ERR_NULL;
     if (hidden_dim <= 0 || n_tokens <= 0 || hidden_stride < hidden_dim) return VIB3_ERR_SHAPE;
     if (x_dtype < X_F32 || x_dtype > X_BF16 || (delta && (delta_dtype < X_F32 || delta_dtype > X_BF16))) return VIB3_ERR_UNSUPPORTED;
     if ((void*)hidden == x_out) return VIB3_ERR_UNSUPPORTED;
     if (delta2 && delta2_stride < hidden_dim) return VIB3_ERR_SHAPE;
-    return launch_norm(hidden, hidden_stride, delta, delta_dtype, delta_stride_bytes, delta2, delta2_stride, weight_f16, eps, center, x_out,
+    return launch_norm(hidden, hidden_stride, delta, delta_dtype, delta_stride_bytes, delta2, delta2_stride, weight_or_null, eps, center, x_out,
                        x_dtype, x_stride_bytes, hidden_dim, n_tokens, (cudaStream_t)stream);
 }
