@@ -102,18 +102,36 @@ def rms_norm_f32(input_f32, output_f32, weight_f16, hidden_dim: int, eps: float,
 EXACT_HOLD = 2   # added to a router launch's exact_order: the producer of x lets its dependents start early
 
 
+def _holds_rows(t: torch.Tensor, T: int, H: int) -> bool:
+    """Whether t has T rows of H contiguous values (a single row may be a vector)."""
+    if t.dim() == 1:
+        return T <= 1 and t.shape[0] >= H and t.stride(0) == 1
+    return t.dim() == 2 and t.shape[0] >= T and t.shape[1] >= H and t.stride(1) == 1
+
+
 def residual_rms_norm(hidden: torch.Tensor, delta, weight_f16, eps: float, x_out: torch.Tensor, stream: Optional[int] = None,
                       delta2=None, center: bool = False, early_dependents: bool = False) -> None:
     """hidden [T, H] fp32 += delta [T, H] + delta2 [T, H] fp32 (either may be None); x_out [T, H] = cast(rms_norm(hidden) *
     weight) with ``weight_f16`` [H] fp16 or, as a tensor of that type, bf16 (None: no weight): one launch.  ``early_dependents``: the next launch of the stream may start while this one runs; it must
     be a router launch with ``EXACT_HOLD`` added to its exact_order argument (see include/vib3_b200.h)."""
+    if hidden.dim() != 2 or hidden.dtype != torch.float32 or hidden.stride(1) != 1:
+        raise ValueError("hidden: fp32 [T, H] with contiguous rows expected")
     T, H = hidden.shape
+    # (the launcher knows addresses and strides only: what is smaller than hidden would be written or read behind its end)
+    if x_out.dtype not in _X_CODES or not _holds_rows(x_out, T, H) or (T > 1 and x_out.stride(0) < H):
+        raise ValueError("x_out: fp32, fp16 or bf16 with room for hidden's rows, each contiguous, expected")
+    if delta is not None and (delta.dtype not in _X_CODES or not _holds_rows(delta, T, H)):
+        raise ValueError("delta: fp32, fp16 or bf16 with a contiguous row for each of hidden's expected")
+    if delta2 is not None and (delta2.dtype != torch.float32 or not _holds_rows(delta2, T, H)):
+        raise ValueError("delta2: fp32 with a contiguous row for each of hidden's expected")
     flags = int(center) | (2 if early_dependents else 0)
     if isinstance(weight_f16, torch.Tensor):
         if weight_f16.dtype == torch.bfloat16:
             flags |= 4
         elif weight_f16.dtype != torch.float16:
             raise ValueError(f"norm weights: fp16 or bf16 expected, got {weight_f16.dtype}")
+        if weight_f16.numel() < H or not weight_f16.is_contiguous():
+            raise ValueError("norm weights: contiguous [H] expected")
     check("residual_rms_norm", lib().vib3_launch_residual_rms_norm(
         _ptr(hidden), hidden.stride(0), _ptr(delta), x_dtype_code(delta) if delta is not None else 0,
         delta.stride(0) * delta.element_size() if delta is not None else 0, _ptr(delta2),
