@@ -104,11 +104,14 @@ class LatentAttention:
         # layers that run one after another may share it
         self.workspace = torch.empty(kernels.latent_attention_workspace_bytes(), dtype=torch.uint8, device=dev) if workspace is None else workspace
 
+    def check_rows(self, rows: int, cache: LatentCache) -> None:
+        if rows > self.max_tokens or rows != cache.step_rows:      # (the slots behind the step's rows are an older step's)
+            raise ValueError(f"the step's {cache.step_rows} rows (sequences * q_len) expected, at most {self.max_tokens}; got {rows}")
+
     def forward(self, x: torch.Tensor, cache: LatentCache, layer: int) -> torch.Tensor:
         """The step that ``cache.begin_step`` laid out.  Returns a view of ``self.out``."""
         sh, T = self.shape, x.shape[0]
-        if T > self.max_tokens or T != cache.step_rows:      # (the slots behind the step's rows are an older step's)
-            raise ValueError(f"x: the step's {cache.step_rows} rows (sequences * q_len) expected, at most {self.max_tokens}; got {T}")
+        self.check_rows(T, cache)
         rows, pos = cache.rows[layer], cache.positions[:T]
         torch.matmul(x, self.w_kv.t(), out=self.kv_in[:T])
         torch.matmul(x, self.w_q.t(), out=self.q_in[:T])
@@ -125,21 +128,36 @@ class DecodeLayer:
     The norms' weights [hidden] are fp16 or bf16."""
 
     def __init__(self, attention: LatentAttention, moe, layer: int, attention_norm: torch.Tensor, moe_norm: torch.Tensor, eps: float = 1e-6):
+        hidden = attention.shape.hidden
+        for norm in (attention_norm, moe_norm):
+            if norm.shape != (hidden,) or norm.dtype not in (torch.float16, torch.bfloat16) or not norm.is_contiguous():
+                raise ValueError(f"norm weights: contiguous fp16 or bf16 [{hidden}] expected")
+        if moe.model.shape.hidden != hidden or not -moe.model.n_layers <= layer < moe.model.n_layers:
+            raise ValueError(f"moe: a decoder with layer {layer} and rows of {hidden} values expected")
         self.attention, self.moe, self.layer = attention, moe, layer
+        self.moe_rows = getattr(moe, "max_tokens", 1)       # of a GroupedDecoder; a MoeDecoder takes one row
         self.attention_norm, self.moe_norm, self.eps = attention_norm, moe_norm, eps
         self.x = torch.zeros(attention.max_tokens, attention.shape.hidden, dtype=attention.w_q.dtype, device=attention.w_q.device)
 
     def forward(self, h: torch.Tensor, cache: LatentCache) -> torch.Tensor:
-        """h [T, hidden] fp32, updated in place."""
+        """h [T, hidden] fp32, updated in place.  Rows, types and decoders that do not fit are refused before h or the cache has changed."""
+        hidden = self.attention.shape.hidden
+        if h.dim() != 2 or h.shape[1] != hidden or h.dtype != torch.float32 or h.stride(1) != 1 or h.stride(0) < hidden:
+            raise ValueError(f"h: fp32 [T, {hidden}] with contiguous rows expected")
+        if h.device != self.x.device or (h.is_cuda and h.get_device() != torch.cuda.current_device()):
+            raise ValueError(f"h: on the layer's device ({self.x.device}), which has to be the current one, expected; got {h.device}")
         T = h.shape[0]
+        self.attention.check_rows(T, cache)
+        if T > self.moe_rows:
+            raise ValueError(f"the MoE decoder takes {self.moe_rows} row(s), got {T} (MoeDecoder takes one; GroupedDecoder takes several)")
+        if not -cache.rows.shape[0] <= self.layer < cache.rows.shape[0]:
+            raise ValueError(f"cache: {cache.rows.shape[0]} layers, none with number {self.layer}")
         x = self.x[:T]
         kernels.residual_rms_norm(h, None, self.attention_norm, self.eps, x)
         delta = self.attention.forward(x, cache, self.layer)
         kernels.residual_rms_norm(h, delta, self.moe_norm, self.eps, x, early_dependents=True)
         if hasattr(self.moe, "max_tokens"):
             self.moe.forward(self.layer, x, out=h, accumulate=True, hold=True)
-        elif T == 1:
-            self.moe.forward_layer(self.layer, x[0], out=h[0], accumulate=True, hold=True)
         else:
-            raise ValueError("MoeDecoder takes one row; GroupedDecoder takes several")
+            self.moe.forward_layer(self.layer, x[0], out=h[0], accumulate=True, hold=True)
         return h
