@@ -19,7 +19,8 @@ from .lib import Vib3Error
 
 class LatentCache:
     """Paged latent rows of ``layers`` layers for up to ``max_sequences`` sequences of up to ``max_pages`` pages each.  One page table
-    serves all layers.  Device buffers of a step (fixed addresses): ``table``, ``lens``, ``positions`` and ``slots``."""
+    serves all layers.  Device buffers of a step (fixed addresses): ``table``, ``lens``, ``positions`` and ``slots`` (behind the step's rows: 0
+    and -1).  A captured step is for steps of its own q_len: with fewer new tokens per sequence give ``begin_step`` that q_len."""
 
     def __init__(self, layers: int, pages: int, page_size: int, max_sequences: int, max_pages: int, dtype: torch.dtype, device,
                  max_tokens: int = 128):
@@ -62,7 +63,11 @@ class LatentCache:
             positions += [0] * pad + list(range(first, first + k))
             slots += [-1] * pad + [own[p // self.page_size] * self.page_size + p % self.page_size for p in range(first, first + k)]
             self.host_lens[b] = first + k
-        n = self.step_rows = len(positions)
+        n, older = len(positions), self.step_rows
+        if n < older:       # a captured step of more rows than this one finds no slots behind it
+            self.positions[n:older].zero_()
+            self.slots[n:older].fill_(-1)
+        self.step_rows = n
         self.positions[:n].copy_(torch.tensor(positions, dtype=torch.int32))
         self.slots[:n].copy_(torch.tensor(slots, dtype=torch.int64))
         if self._table_changed:
@@ -105,7 +110,7 @@ class LatentAttention:
         self.workspace = torch.empty(kernels.latent_attention_workspace_bytes(), dtype=torch.uint8, device=dev) if workspace is None else workspace
 
     def check_rows(self, rows: int, cache: LatentCache) -> None:
-        if rows > self.max_tokens or rows != cache.step_rows:      # (the slots behind the step's rows are an older step's)
+        if rows > self.max_tokens or rows != cache.step_rows:
             raise ValueError(f"the step's {cache.step_rows} rows (sequences * q_len) expected, at most {self.max_tokens}; got {rows}")
 
     def forward(self, x: torch.Tensor, cache: LatentCache, layer: int) -> torch.Tensor:
