@@ -35,9 +35,13 @@ constexpr int kAttThreads = 384;                          // copies, S, O, (none
 constexpr int kSoftmaxThreads = 256;
 constexpr int kTmemCols = 512, kSCol = 256, kQCol = 320;  // O^T: 4 x 64 columns, S: 64, Q: 6 x 32
 static_assert(kQCol + 32 * kQTmemChunks <= kTmemCols, "tensor memory");
-// The reference m of a row follows its maximum only when that has grown by more than 2^8: exp(s - m) then stays below 256, the
-// 16-bit weights keep their relative precision, and the accumulator is rescaled a few times per sequence instead of per tile.
+// The reference m of a row follows its maximum only when that has grown by more than 2^8, so that the accumulator is rescaled a few times per
+// sequence instead of per tile.  The weights exp(s - m) are rounded to the operands' 16-bit type, since an MMA takes one type for both; their
+// sum l has them unrounded.  A bf16 weight is off by 2^-8 of itself however small it is.  fp16 is subnormal below 2^-14 and has nothing below
+// 2^-25, so there m stays 2^7 below the maximum and the row's largest weight lies between 2^7 and 2^15 (of 65504): a weight is off by 2^-11 of
+// itself or 2^-32 of the largest, and tens of thousands of keys beside a dominating one keep their share.
 constexpr float kLazy = 8.0f;
+template <typename T> constexpr float kLead = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 constexpr int kMaxGrid = 160;                             // CTAs that the workspace has room for
 constexpr size_t kPartFloats = (size_t)kTileRows * kRank;
 
@@ -501,6 +505,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
         };
         if (stid == 0 && !a.by_item) a.made_of[blockIdx.x] = make_int4(0, 0, 0, 0);
         // A round: the next piece's Q requested, the results of the piece before, with Q put in place half way, the next one's tiles.
+        constexpr float kAhead = kLead<T> + kLazy;     // of a row's maximum before its reference
         float m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f;
         long long token0 = 0;
         Piece next;
@@ -631,7 +636,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
                     x0 = fmaxf(x0, fmaxf(v[4 * x], v[4 * x + 1]));
                     x1 = fmaxf(x1, fmaxf(v[4 * x + 2], v[4 * x + 3]));
                 }
-                if (softmax_any(x0 > m0 + kLazy || x1 > m1 + kLazy || !ok)) {
+                if (softmax_any(x0 > m0 + kAhead || x1 > m1 + kAhead || !ok)) {
                     // a reference moves: the rows' maxima over both teams, then O's rows times exp2(old - new)
                     ok = !softmax_any(!ok);
                     if (!ok) break;
@@ -648,14 +653,16 @@ __global__ void __launch_bounds__(kAttThreads, 1) latent_attention_kernel(const 
                     x0 = fmaxf(x0, sh.team[team ^ 1][r0]);
                     x1 = fmaxf(x1, sh.team[team ^ 1][r1]);
                     float f0 = 1.f, f1 = 1.f;
-                    if (x0 > m0 + kLazy) {
-                        f0 = m0 == -INFINITY ? 1.f : ex2(m0 - x0);
-                        m0 = x0;
+                    if (x0 > m0 + kAhead) {
+                        const float m = x0 - kLead<T>;
+                        f0 = m0 == -INFINITY ? 1.f : ex2(m0 - m);
+                        m0 = m;
                         l0 *= f0;
                     }
-                    if (x1 > m1 + kLazy) {
-                        f1 = m1 == -INFINITY ? 1.f : ex2(m1 - x1);
-                        m1 = x1;
+                    if (x1 > m1 + kAhead) {
+                        const float m = x1 - kLead<T>;
+                        f1 = m1 == -INFINITY ? 1.f : ex2(m1 - m);
+                        m1 = m;
                         l1 *= f1;
                     }
                     if (t > p.t0) {
