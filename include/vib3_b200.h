@@ -369,7 +369,7 @@ int vib3_launch_moe_grouped_int4(void* handle, const void* x, int x_dtype, int x
  * cache (cuda/src/kernels.cu:1570, :1624, :1679, :1709); these launchers take the tokens of a step and a paged cache.
  * Strides are in ELEMENTS and multiples of 16 bytes, pointers 16-byte aligned (VIB3_ERR_ALIGN); the last dimension of every
  * matrix is contiguous; dtypes are VIB3_X_F16 or VIB3_X_BF16, one for all 16-bit operands of a call.  n_tokens, batch or q_len 0:
- * nothing is launched.  The launches are programmatic dependents that read nothing before their predecessor has finished.
+ * nothing is launched, and the addresses of what has no rows then may be null.  The launches are programmatic dependents that read nothing before their predecessor has finished.
  * inv_freq: 32 doubles on the device, one per pair of position values; the angle position * inv_freq[i] is formed in 64 bits.
  * pairs != 0: value 2 i turns with value 2 i + 1; 0: value i with value i + 32.  rope_scale multiplies the rotated values.
  * status (may be NULL): one int on the device that a launch sets bits of; VIB3_STATUS_TIMEOUT, from every launch but the append, means

@@ -117,6 +117,8 @@ class LatentAttention:
         """The step that ``cache.begin_step`` laid out.  Returns a view of ``self.out``."""
         sh, T = self.shape, x.shape[0]
         self.check_rows(T, cache)
+        if T == 0:
+            return self.out[:0]
         rows, pos = cache.rows[layer], cache.positions[:T]
         torch.matmul(x, self.w_kv.t(), out=self.kv_in[:T])
         torch.matmul(x, self.w_q.t(), out=self.q_in[:T])
@@ -157,6 +159,8 @@ class DecodeLayer:
             raise ValueError(f"the MoE decoder takes {self.moe_rows} row(s), got {T} (MoeDecoder takes one; GroupedDecoder takes several)")
         if not -cache.rows.shape[0] <= self.layer < cache.rows.shape[0]:
             raise ValueError(f"cache: {cache.rows.shape[0]} layers, none with number {self.layer}")
+        if T == 0:
+            return h
         x = self.x[:T]
         kernels.residual_rms_norm(h, None, self.attention_norm, self.eps, x)
         delta = self.attention.forward(x, cache, self.layer)

@@ -922,7 +922,8 @@ extern "C" int vib3_launch_latent_attention_paged(const void* q, long long q_tok
                                                   int batch, int q_len, int heads, float scale, int dtype, void* out,
                                                   long long out_token_stride, long long out_head_stride, float* lse_or_null,
                                                   void* workspace, size_t workspace_bytes, int* status, void* stream) {
-    if (!q || !cache || !page_table || !seq_lens || !out || !workspace) return VIB3_ERR_NULL;
+    // (without rows or sequences the address of an empty tensor is null)
+    if ((batch != 0 && (!page_table || !seq_lens || (q_len != 0 && (!q || !out)))) || !cache || !workspace) return VIB3_ERR_NULL;
     if (dtype != L_F16 && dtype != L_BF16) return VIB3_ERR_UNSUPPORTED;
     if (page_size % 8) return VIB3_ERR_UNSUPPORTED;
     // (the copying warp looks up table entries for 32 boxes at once, up to 2048 keys beyond the length, and key numbers have 32 bits)

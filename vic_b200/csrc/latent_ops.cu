@@ -384,7 +384,7 @@ extern "C" int vib3_launch_latent_append_paged(const void* kv, int kv_dtype, lon
                                                const int* positions, const long long* slots, const double* inv_freq, float rope_scale,
                                                int pairs, int n_tokens, void* cache, int cache_dtype, long long num_pages, int page_size,
                                                long long page_stride, long long row_stride, int* status, void* stream) {
-    if (!kv || !positions || !slots || !inv_freq || !cache) return VIB3_ERR_NULL;
+    if ((n_tokens != 0 && (!kv || !positions || !slots)) || !inv_freq || !cache) return VIB3_ERR_NULL;     // (no tokens: an empty tensor's address is null)
     if (n_tokens < 0 || n_tokens > kLatentMaxTokens || num_pages <= 0 || page_size <= 0) return VIB3_ERR_COUNT;
     if (kv_dtype < L_F32 || kv_dtype > L_BF16 || (cache_dtype != L_F16 && cache_dtype != L_BF16)) return VIB3_ERR_UNSUPPORTED;
     const int per16 = kv_dtype == L_F32 ? 4 : 8;
@@ -409,7 +409,7 @@ extern "C" int vib3_launch_latent_append_paged(const void* kv, int kv_dtype, lon
 }
 
 static int check_heads(const HeadArgs& g, int dtype, int in_width, int out_width) {
-    if (!g.a || !g.w || !g.out) return VIB3_ERR_NULL;
+    if ((g.n_tokens != 0 && (!g.a || !g.out)) || !g.w) return VIB3_ERR_NULL;
     if (g.n_tokens < 0 || g.n_tokens > kLatentMaxTokens / 4 || g.heads <= 0 || g.heads > kLatentMaxHeads) return VIB3_ERR_COUNT;
     if (dtype != L_F16 && dtype != L_BF16) return VIB3_ERR_UNSUPPORTED;
     if (g.dim < 16 || g.dim > 256 || g.dim % 16) return VIB3_ERR_UNSUPPORTED;
@@ -428,7 +428,7 @@ extern "C" int vib3_launch_latent_query(const void* q, long long q_token_stride,
                                         int dtype, int* status, void* stream) {
     HeadArgs g{q, q_token_stride, q_head_stride, w_uk, w_head_stride, out, out_token_stride, out_head_stride, n_tokens, heads, nope,
                positions, inv_freq, rope_scale, pairs, status};
-    if (!positions || !inv_freq) return VIB3_ERR_NULL;
+    if ((n_tokens != 0 && !positions) || !inv_freq) return VIB3_ERR_NULL;
     const int e = check_heads(g, dtype, nope + kRope, kLatentRow);
     if (e) return e;
     if (n_tokens == 0) return VIB3_OK;
