@@ -385,6 +385,8 @@ def latent_append(kv: torch.Tensor, norm_weight: Optional[torch.Tensor], eps: fl
         raise ValueError("inv_freq: contiguous float64 [32] expected")
     if norm_weight is not None and (norm_weight.shape != (LATENT_RANK,) or norm_weight.dtype != dt or not norm_weight.is_contiguous()):
         raise ValueError("norm_weight: contiguous [512] of the cache's dtype expected")
+    if status is not None and (status.dtype != _I32 or status.numel() == 0):
+        raise ValueError("status: int32 [1] expected")
     launch = (_latent or _bind_latent())[0]
     dev = _current_device()     # (a launch on another one would read through a foreign context)
     if not (dev == kv.get_device() == cache.get_device() == slots.get_device() == positions.get_device() == inv_freq.get_device()
@@ -419,6 +421,8 @@ def latent_query(q: torch.Tensor, w_uk: torch.Tensor, positions: torch.Tensor, i
         raise ValueError("inv_freq: contiguous float64 [32] expected")
     if (dt != torch.bfloat16 and dt != torch.float16) or w_uk.dtype != dt or out.dtype != dt:
         raise ValueError("one dtype, fp16 or bf16, expected")
+    if status is not None and (status.dtype != _I32 or status.numel() == 0):
+        raise ValueError("status: int32 [1] expected")
     launch = (_latent or _bind_latent())[1]
     dev = _current_device()     # (a launch on another one would read through a foreign context)
     if not (dev == q.get_device() == w_uk.get_device() == positions.get_device() == inv_freq.get_device() == out.get_device()
@@ -447,6 +451,8 @@ def latent_value(o: torch.Tensor, w_uv: torch.Tensor, out: torch.Tensor, status:
         raise ValueError("out: [T, H, value] with contiguous rows expected")
     if (dt != torch.bfloat16 and dt != torch.float16) or w_uv.dtype != dt or out.dtype != dt:
         raise ValueError("one dtype, fp16 or bf16, expected")
+    if status is not None and (status.dtype != _I32 or status.numel() == 0):
+        raise ValueError("status: int32 [1] expected")
     launch = (_latent or _bind_latent())[2]
     dev = _current_device()     # (a launch on another one would read through a foreign context)
     if not (dev == o.get_device() == w_uv.get_device() == out.get_device() == (o if status is None else status).get_device()):
@@ -491,6 +497,8 @@ def latent_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Ten
         raise ValueError("one dtype, fp16 or bf16, expected")
     if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise ValueError("workspace: contiguous uint8 expected")
+    if status is not None and (status.dtype != _I32 or status.numel() == 0):
+        raise ValueError("status: int32 [1] expected")
     launch = (_latent or _bind_latent())[3]
     dev = _current_device()     # (a launch on another one would read through a foreign context)
     if not (dev == q.get_device() == cache.get_device() == page_table.get_device() == seq_lens.get_device() == out.get_device()
