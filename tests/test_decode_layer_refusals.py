@@ -86,3 +86,16 @@ def test_decoders_that_do_not_fit_are_refused_when_the_layer_is_made(monkeypatch
     with pytest.raises(ValueError, match="cache"):           # (the cache has one layer)
         second.forward(torch.ones(3, 64), cache)
     assert launched == []
+
+
+def test_frequencies_of_another_form_are_refused_when_the_layer_is_made():
+    from vic_b200.attention import LatentAttention
+    from vic_b200.core_types import LatentShape
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    sh = LatentShape("small", 64, 2, 16, 16, 10000.0, 1e-6)
+    make = lambda f: LatentAttention(sh, z(160, 64), z(576, 64), z(512), z(2, 32, 512), z(64, 32), inv_freq=f)  # noqa: E731
+    for bad in (torch.ones(32), torch.ones(64, dtype=torch.float64), torch.ones(64, dtype=torch.float64)[::2], torch.ones(1, 32, dtype=torch.float64)):
+        with pytest.raises(ValueError, match="inv_freq"):
+            make(bad)
+    good = torch.rand(32, dtype=torch.float64)
+    assert make(good).inv_freq is good and make(None).inv_freq[1].item() == pytest.approx(10000.0 ** (-1 / 32), rel=1e-15)

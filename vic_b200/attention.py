@@ -88,17 +88,22 @@ class LatentAttention:
     """One layer: x [T, hidden] -> output [T, hidden], T = sequences * q_len rows in the cache's order.
 
     ``w_q`` [heads * (nope + 64), hidden], ``w_kv`` [576, hidden], ``kv_norm`` [512], ``kv_b`` [heads, nope + value, 512] (the heads' key
-    and value matrices), ``w_o`` [hidden, heads * value]; one dtype, fp16 or bf16."""
+    and value matrices), ``w_o`` [hidden, heads * value]; one dtype, fp16 or bf16.  ``inv_freq`` [32] float64: the angles per position, where
+    they are not the powers of the shape's rope_theta."""
 
     def __init__(self, shape: LatentShape, w_q: torch.Tensor, w_kv: torch.Tensor, kv_norm: torch.Tensor, kv_b: torch.Tensor,
-                 w_o: torch.Tensor, max_tokens: int = 128, workspace: Optional[torch.Tensor] = None):
+                 w_o: torch.Tensor, max_tokens: int = 128, workspace: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None):
         dev, dt, H = w_q.device, w_q.dtype, shape.heads
         if w_q.shape != (H * (shape.nope + LATENT_ROPE), shape.hidden) or w_kv.shape != (LATENT_ROW, shape.hidden) or kv_norm.shape != (LATENT_RANK,) or \
                 kv_b.shape != (H, shape.nope + shape.value, LATENT_RANK) or w_o.shape != (shape.hidden, H * shape.value):
             raise ValueError("weights do not have the layer's shape")
         self.shape, self.max_tokens = shape, max_tokens
         self.w_q, self.w_kv, self.kv_norm, self.kv_b, self.w_o = w_q, w_kv, kv_norm, kv_b, w_o
-        self.inv_freq = shape.rope_theta ** (-torch.arange(0, LATENT_ROPE, 2, dtype=torch.float64, device=dev) / LATENT_ROPE)
+        if inv_freq is None:
+            inv_freq = shape.rope_theta ** (-torch.arange(0, LATENT_ROPE, 2, dtype=torch.float64, device=dev) / LATENT_ROPE)
+        elif inv_freq.shape != (LATENT_ROPE // 2,) or inv_freq.dtype != torch.float64 or inv_freq.device != dev or not inv_freq.is_contiguous():
+            raise ValueError(f"inv_freq: contiguous float64 [32] on {dev} expected")
+        self.inv_freq = inv_freq
         self.q_in = torch.zeros(max_tokens, H * (shape.nope + LATENT_ROPE), dtype=dt, device=dev)
         self.kv_in = torch.zeros(max_tokens, LATENT_ROW, dtype=dt, device=dev)
         self.q = torch.zeros(max_tokens, H, LATENT_ROW, dtype=dt, device=dev)
@@ -122,8 +127,10 @@ class LatentAttention:
         rows, pos = cache.rows[layer], cache.positions[:T]
         torch.matmul(x, self.w_kv.t(), out=self.kv_in[:T])
         torch.matmul(x, self.w_q.t(), out=self.q_in[:T])
-        kernels.latent_append(self.kv_in[:T], self.kv_norm, sh.eps, pos, cache.slots[:T], self.inv_freq, rows, status=self.status)
-        kernels.latent_query(self.q_in[:T].view(T, sh.heads, sh.nope + LATENT_ROPE), self.kv_b[:, :sh.nope], pos, self.inv_freq, self.q[:T], status=self.status)
+        kernels.latent_append(self.kv_in[:T], self.kv_norm, sh.eps, pos, cache.slots[:T], self.inv_freq, rows,
+                              pairs=sh.pairs, rope_scale=sh.rope_scale, status=self.status)
+        kernels.latent_query(self.q_in[:T].view(T, sh.heads, sh.nope + LATENT_ROPE), self.kv_b[:, :sh.nope], pos, self.inv_freq, self.q[:T],
+                             pairs=sh.pairs, rope_scale=sh.rope_scale, status=self.status)
         kernels.latent_attention(self.q[:T], rows, cache.table, cache.lens, sh.scale, self.o[:T], workspace=self.workspace, status=self.status)
         kernels.latent_value(self.o[:T], self.kv_b[:, sh.nope:], self.v[:T], status=self.status)
         torch.matmul(self.v[:T].view(T, sh.heads * sh.value), self.w_o.t(), out=self.out[:T])

@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import Optional
 
 PAGE_SIZE = 2 * 1024 * 1024      # types.rs:14
 MAX_EXPERTS = 512                # types.rs:20
@@ -120,11 +121,15 @@ class LatentShape:
     value: int               # width of a head's output
     rope_theta: float
     eps: float
+    softmax_scale: Optional[float] = None    # None: 1 / sqrt(nope + 64); models with scaled positions multiply it
+    rope_scale: float = 1.0                  # of the rotated values, of queries and cache rows alike
+    pairs: bool = True                       # neighbouring values turn together; False: values 32 apart
 
     @property
     def scale(self) -> float:
-        return (self.nope + 64) ** -0.5
+        return (self.nope + 64) ** -0.5 if self.softmax_scale is None else self.softmax_scale
 
 
-# The attention sublayer that goes with KIMI: 64 heads of 128 + 64 and 128 over a latent of 512
+# The sizes of the attention sublayer that goes with KIMI: 64 heads of 128 + 64 and 128 over a latent of 512, positions unscaled.  A checkpoint's
+# own scaling of positions is given by replacing softmax_scale and rope_scale, and by LatentAttention's inv_freq.
 KIMI_LATENT = LatentShape("kimi-k2.5", 7168, 64, 128, 128, 50000.0, 1e-6)
