@@ -5,7 +5,7 @@ import torch
 
 class Model:
     def __init__(self, hidden=64, n_layers=1):
-        self.shape, self.n_layers = type("Shape", (), {"hidden": hidden}), n_layers
+        self.shape, self.n_layers = type("Shape", (), {"hidden": hidden, "num_experts": 6}), n_layers
 
 
 class Grouped:
@@ -99,3 +99,13 @@ def test_frequencies_of_another_form_are_refused_when_the_layer_is_made():
             make(bad)
     good = torch.rand(32, dtype=torch.float64)
     assert make(good).inv_freq is good and make(None).inv_freq[1].item() == pytest.approx(10000.0 ** (-1 / 32), rel=1e-15)
+
+
+def test_selection_biases_of_another_form_are_refused_when_the_layer_is_made(monkeypatch):
+    from vic_b200.attention import DecodeLayer
+    layer, _, _ = parts(monkeypatch, Grouped(128), 24, 12)
+    norm = torch.ones(64, dtype=torch.bfloat16)
+    for bad in (torch.zeros(5), torch.zeros(6, dtype=torch.bfloat16), torch.zeros(12)[::2], torch.zeros(1, 6)):
+        with pytest.raises(ValueError, match="selection_bias"):
+            DecodeLayer(layer.attention, layer.moe, 0, norm, norm, selection_bias=bad)
+    assert DecodeLayer(layer.attention, layer.moe, 0, norm, norm, selection_bias=torch.zeros(6)).selection_bias is not None

@@ -139,15 +139,20 @@ class LatentAttention:
 
 class DecodeLayer:
     """h += attention(norm(h)), h += moe(norm(h)) for a step's rows: ``moe`` is a MoeDecoder (one row) or a GroupedDecoder.
-    The norms' weights [hidden] are fp16 or bf16."""
+    The norms' weights [hidden] are fp16 or bf16.  ``selection_bias`` [experts] fp32 is added to the router's scores for the selection only."""
 
-    def __init__(self, attention: LatentAttention, moe, layer: int, attention_norm: torch.Tensor, moe_norm: torch.Tensor, eps: float = 1e-6):
+    def __init__(self, attention: LatentAttention, moe, layer: int, attention_norm: torch.Tensor, moe_norm: torch.Tensor, eps: float = 1e-6,
+                 selection_bias: Optional[torch.Tensor] = None):
         hidden = attention.shape.hidden
         for norm in (attention_norm, moe_norm):
             if norm.shape != (hidden,) or norm.dtype not in (torch.float16, torch.bfloat16) or not norm.is_contiguous():
                 raise ValueError(f"norm weights: contiguous fp16 or bf16 [{hidden}] expected")
         if moe.model.shape.hidden != hidden or not -moe.model.n_layers <= layer < moe.model.n_layers:
             raise ValueError(f"moe: a decoder with layer {layer} and rows of {hidden} values expected")
+        if selection_bias is not None and (selection_bias.shape != (moe.model.shape.num_experts,) or selection_bias.dtype != torch.float32
+                                           or not selection_bias.is_contiguous() or selection_bias.device != attention.w_q.device):
+            raise ValueError(f"selection_bias: contiguous fp32 [{moe.model.shape.num_experts}] on {attention.w_q.device} expected")
+        self.selection_bias = selection_bias
         self.attention, self.moe, self.layer = attention, moe, layer
         self.moe_rows = getattr(moe, "max_tokens", 1)       # of a GroupedDecoder; a MoeDecoder takes one row
         self.attention_norm, self.moe_norm, self.eps = attention_norm, moe_norm, eps
@@ -173,7 +178,7 @@ class DecodeLayer:
         delta = self.attention.forward(x, cache, self.layer)
         kernels.residual_rms_norm(h, delta, self.moe_norm, self.eps, x, early_dependents=True)
         if hasattr(self.moe, "max_tokens"):
-            self.moe.forward(self.layer, x, out=h, accumulate=True, hold=True)
+            self.moe.forward(self.layer, x, out=h, accumulate=True, hold=True, bias=self.selection_bias)
         else:
-            self.moe.forward_layer(self.layer, x[0], out=h[0], accumulate=True, hold=True)
+            self.moe.forward_layer(self.layer, x[0], out=h[0], accumulate=True, bias=self.selection_bias, hold=True)
         return h

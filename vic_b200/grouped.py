@@ -104,11 +104,12 @@ class GroupedDecoder:
         return out
 
     def forward(self, layer: int, xs: torch.Tensor, out: Optional[torch.Tensor] = None, accumulate: bool = False,
-                logit_offset: Optional[torch.Tensor] = None, hold: bool = False) -> torch.Tensor:
-        """xs [T, H] (bf16 / fp16 / fp32, T <= max_tokens) -> [T, H] fp32; routing left in self.ids / self.weights."""
+                logit_offset: Optional[torch.Tensor] = None, hold: bool = False, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """xs [T, H] (bf16 / fp16 / fp32, T <= max_tokens) -> [T, H] fp32; routing left in self.ids / self.weights.  ``bias`` [E] fp32 is
+        added to the scores for the selection only."""
         if xs.shape[0] > self.max_tokens:
             raise ValueError("more tokens than the decoder was built for")
-        self.route(layer, xs, logit_offset, hold=hold)
+        self.route(layer, xs, logit_offset, bias, hold=hold)
         return self.experts(layer, xs, out, accumulate)
 
 
