@@ -109,3 +109,17 @@ def test_selection_biases_of_another_form_are_refused_when_the_layer_is_made(mon
         with pytest.raises(ValueError, match="selection_bias"):
             DecodeLayer(layer.attention, layer.moe, 0, norm, norm, selection_bias=bad)
     assert DecodeLayer(layer.attention, layer.moe, 0, norm, norm, selection_bias=torch.zeros(6)).selection_bias is not None
+
+
+def test_queries_of_low_rank_that_do_not_fit_are_refused_when_the_layer_is_made():
+    from vic_b200.attention import LatentAttention
+    from vic_b200.core_types import LatentShape
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    sh = LatentShape("small", 64, 2, 16, 16, 10000.0, 1e-6)
+    make = lambda w_q, **k: LatentAttention(sh, w_q, z(576, 64), z(512), z(2, 32, 512), z(64, 32), **k)  # noqa: E731
+    make(z(160, 24), q_down=z(24, 64), q_norm=z(24))
+    for w_q, k in ((z(160, 24), {}), (z(160, 64), dict(q_down=z(24, 64), q_norm=z(24))), (z(160, 24), dict(q_down=z(24, 64))), (z(160, 64), dict(q_norm=z(64))),
+                   (z(160, 24), dict(q_down=z(24, 32), q_norm=z(24))), (z(160, 24), dict(q_down=z(24, 64).half(), q_norm=z(24))),
+                   (z(160, 24), dict(q_down=z(24, 64), q_norm=z(23))), (z(160, 24), dict(q_down=z(24, 64), q_norm=z(24).float()))):
+        with pytest.raises(ValueError):
+            make(w_q, **k)

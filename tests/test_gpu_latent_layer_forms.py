@@ -49,3 +49,28 @@ def test_rotation_and_scale_are_the_layers(cuda_dev, pairs, rope_scale, softmax_
         ds = 576 * 2.0 ** -23 * err + 2.0 ** -20
         assert_rounded(att.o[:T], want, (2 * ds + u(torch.bfloat16) + 64 * 2.0 ** -24).unsqueeze(-1) * mag)
     assert int(att.status) == 0
+
+
+@pytest.mark.parametrize("rank,norm_dtype", [(96, torch.bfloat16), (1536, torch.float16)])
+def test_queries_of_low_rank(cuda_dev, rank, norm_dtype):
+    """norm(x q_down^T) w_q^T: each product within its operands' and its own rounding (2^-8 of the magnitudes' sum covers any order of additions)."""
+    from tests.test_gpu_latent import assert_rounded, attention64, u
+    g = torch.Generator(device=cuda_dev).manual_seed(9)
+    down = (torch.randn(rank, 256, generator=g, device=cuda_dev) / 16).to(torch.bfloat16)
+    norm = (1 + 0.2 * torch.randn(rank, generator=g, device=cuda_dev)).to(norm_dtype)
+    att, cache, g = layer(cuda_dev, shape_of(), q_width=rank, q_down=down, q_norm=norm)
+    for new in ([5, 8, 2], [1, 1, 1]):
+        cache.begin_step(new)
+        T = cache.step_rows
+        x = torch.randn(T, 256, generator=g, device=cuda_dev).to(torch.bfloat16)
+        att.forward(x, cache, 0)
+        low = x.double() @ down.double().T
+        assert bool(((att.q_low32[:T].double() - low).abs() <= 2.0 ** -8 * (x.double().abs() @ down.double().abs().T)).all())
+        low = att.q_low32[:T].double()
+        low = low / (low.square().mean(1, keepdim=True) + 1e-6).sqrt() * norm.double()
+        assert_rounded(att.q_low[:T], low, 64 * 2.0 ** -24 * low.abs())
+        a, b = att.q_low[:T].double(), att.w_q.double()
+        assert bool(((att.q_in[:T].double() - a @ b.T).abs() <= 2.0 ** -8 * (a.abs() @ b.abs().T)).all())
+        want, _, mag, err = attention64(att.q[:T], cache.rows[0], cache.table, cache.lens, 128 ** -0.5)
+        assert_rounded(att.o[:T], want, (2 * (576 * 2.0 ** -23 * err + 2.0 ** -20) + u(torch.bfloat16) + 64 * 2.0 ** -24).unsqueeze(-1) * mag)
+    assert int(att.status) == 0

@@ -89,12 +89,26 @@ class LatentAttention:
 
     ``w_q`` [heads * (nope + 64), hidden], ``w_kv`` [576, hidden], ``kv_norm`` [512], ``kv_b`` [heads, nope + value, 512] (the heads' key
     and value matrices), ``w_o`` [hidden, heads * value]; one dtype, fp16 or bf16.  ``inv_freq`` [32] float64: the angles per position, where
-    they are not the powers of the shape's rope_theta."""
+    they are not the powers of the shape's rope_theta.  Queries of low rank: ``q_down`` [q_rank, hidden] and ``q_norm`` [q_rank], and ``w_q``
+    [heads * (nope + 64), q_rank] then takes norm(x q_down^T)."""
 
     def __init__(self, shape: LatentShape, w_q: torch.Tensor, w_kv: torch.Tensor, kv_norm: torch.Tensor, kv_b: torch.Tensor,
-                 w_o: torch.Tensor, max_tokens: int = 128, workspace: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None):
+                 w_o: torch.Tensor, max_tokens: int = 128, workspace: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None,
+                 q_down: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None):
         dev, dt, H = w_q.device, w_q.dtype, shape.heads
-        if w_q.shape != (H * (shape.nope + LATENT_ROPE), shape.hidden) or w_kv.shape != (LATENT_ROW, shape.hidden) or kv_norm.shape != (LATENT_RANK,) or \
+        if (q_down is None) != (q_norm is None):
+            raise ValueError("q_down and q_norm: both or neither")
+        q_width = shape.hidden
+        if q_down is not None:
+            if q_down.dim() != 2 or q_down.shape[1] != shape.hidden or q_down.dtype != dt:
+                raise ValueError(f"q_down: [q_rank, {shape.hidden}] of the layer's dtype expected")
+            q_width = q_down.shape[0]
+            if q_norm.shape != (q_width,) or q_norm.dtype not in (torch.float16, torch.bfloat16) or not q_norm.is_contiguous():
+                raise ValueError(f"q_norm: contiguous fp16 or bf16 [{q_width}] expected")
+            self.q_low32 = torch.zeros(max_tokens, q_width, device=dev)
+            self.q_low = torch.zeros(max_tokens, q_width, dtype=dt, device=dev)
+        self.q_down, self.q_norm = q_down, q_norm
+        if w_q.shape != (H * (shape.nope + LATENT_ROPE), q_width) or w_kv.shape != (LATENT_ROW, shape.hidden) or kv_norm.shape != (LATENT_RANK,) or \
                 kv_b.shape != (H, shape.nope + shape.value, LATENT_RANK) or w_o.shape != (shape.hidden, H * shape.value):
             raise ValueError("weights do not have the layer's shape")
         self.shape, self.max_tokens = shape, max_tokens
@@ -126,7 +140,12 @@ class LatentAttention:
             return self.out[:0]
         rows, pos = cache.rows[layer], cache.positions[:T]
         torch.matmul(x, self.w_kv.t(), out=self.kv_in[:T])
-        torch.matmul(x, self.w_q.t(), out=self.q_in[:T])
+        q = x
+        if self.q_down is not None:
+            q = torch.matmul(x, self.q_down.t(), out=self.q_low[:T])
+            self.q_low32[:T].copy_(q)
+            kernels.residual_rms_norm(self.q_low32[:T], None, self.q_norm, sh.eps, q)
+        torch.matmul(q, self.w_q.t(), out=self.q_in[:T])
         kernels.latent_append(self.kv_in[:T], self.kv_norm, sh.eps, pos, cache.slots[:T], self.inv_freq, rows,
                               pairs=sh.pairs, rope_scale=sh.rope_scale, status=self.status)
         kernels.latent_query(self.q_in[:T].view(T, sh.heads, sh.nope + LATENT_ROPE), self.kv_b[:, :sh.nope], pos, self.inv_freq, self.q[:T],

@@ -131,5 +131,6 @@ class LatentShape:
 
 
 # The sizes of the attention sublayer that goes with KIMI: 64 heads of 128 + 64 and 128 over a latent of 512, positions unscaled.  A checkpoint's
-# own scaling of positions is given by replacing softmax_scale and rope_scale, and by LatentAttention's inv_freq.
+# own scaling of positions is given by replacing softmax_scale and rope_scale, and by LatentAttention's inv_freq; its queries' low rank
+# by LatentAttention's q_down and q_norm.
 KIMI_LATENT = LatentShape("kimi-k2.5", 7168, 64, 128, 128, 50000.0, 1e-6)
