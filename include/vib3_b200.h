@@ -406,7 +406,9 @@ int vib3_launch_latent_value(const void* o, long long o_token_stride, long long 
  * [0, num_pages), or whose table entry lies beyond max_pages_per_seq, is left out and VIB3_STATUS_MISSING_PAGE is set.  Rows of the cache behind a
  * sequence's length may hold anything; those within it are read by every token of the call that shares a tile with them and have to be
  * finite.  page_size: a multiple of 8; max_pages_per_seq * page_size <=
- * 2^31 - 4096; heads <= 128; batch * q_len <= 1048576.  workspace: at least
+ * 2^31 - 4096; heads <= 128; batch * q_len <= 1048576; and, since the kernel counts 64-key tiles in 32 bits, batch * b *
+ * (max_pages_per_seq * page_size / 64 + 5) <= 2^31 - 256, where b = ceil(q_len * heads / 64) is taken as 1 up to 8 (VIB3_ERR_COUNT; the lengths are not
+ * known here, so the table's width counts).  workspace: at least
  * vib3_latent_attention_workspace_bytes(), contents irrelevant; calls sharing a workspace must not overlap. */
 size_t vib3_latent_attention_workspace_bytes(void);
 int vib3_launch_latent_attention_paged(const void* q, long long q_token_stride, long long q_head_stride, const void* cache,

@@ -941,7 +941,6 @@ extern "C" int vib3_launch_latent_attention_paged(const void* q, long long q_tok
         return VIB3_ERR_ALIGN;
     if (workspace_bytes < kAttWorkspace) return VIB3_ERR_CAPACITY;
     if (batch == 0 || q_len == 0) return VIB3_OK;
-    if (!tensor_map_encoder()) return VIB3_ERR_UNSUPPORTED;
 
     AttentionArgs a;
     a.q = q; a.q_token = q_token_stride; a.q_head = q_head_stride;
@@ -972,6 +971,7 @@ extern "C" int vib3_launch_latent_attention_paged(const void* q, long long q_tok
     a.min_cost = kMinCost;
     const int grid = sms / a.lanes * a.lanes;
 
+    if (!tensor_map_encoder()) return VIB3_ERR_UNSUPPORTED;
     CUtensorMap map;
     if (!map_3d(&map, dtype, cache, kLatentRow, page_size, num_pages, row_stride, page_stride, a.box_rows, 1))
         return VIB3_ERR_SHAPE;
