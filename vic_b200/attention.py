@@ -42,8 +42,9 @@ class LatentCache:
         self._free = list(range(pages - 1, -1, -1))
 
     def begin_step(self, new_tokens: Sequence[int], q_len: Optional[int] = None) -> None:
-        """Sequence b gets new_tokens[b] tokens (0: it takes no part): pages for them, their positions and slots, the lengths with
-        them.  A step's rows are q_len (default: the largest count) per sequence, the new tokens last; the rows before them are padding."""
+        """Sequence b gets new_tokens[b] tokens (0: none): pages for them, their positions and slots, the lengths with them.
+        A step's rows are q_len (default: the largest count) per sequence, the new tokens last.  The rows before them are padding: nothing is
+        stored of them, but they attend to what their sequence has (and so cost its cache's bytes), and what comes of them means nothing."""
         if len(new_tokens) != self.max_sequences:
             raise ValueError(f"{self.max_sequences} counts expected")
         q_len = max(new_tokens) if q_len is None else q_len

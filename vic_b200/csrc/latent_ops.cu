@@ -408,7 +408,7 @@ extern "C" int vib3_launch_latent_append_paged(const void* kv, int kv_dtype, lon
     return launch_latent(latent_append_kernel<__nv_bfloat16, __nv_bfloat16>, grid, threads, 0, st, a);
 }
 
-static int check_heads(const HeadArgs& g, int dtype, int in_width, int out_width) {
+static int check_heads(const HeadArgs& g, int dtype, int out_width) {
     if ((g.n_tokens != 0 && (!g.a || !g.out)) || !g.w) return VIB3_ERR_NULL;
     if (g.n_tokens < 0 || g.n_tokens > kLatentMaxTokens / 4 || g.heads <= 0 || g.heads > kLatentMaxHeads) return VIB3_ERR_COUNT;
     if (dtype != L_F16 && dtype != L_BF16) return VIB3_ERR_UNSUPPORTED;
@@ -416,7 +416,6 @@ static int check_heads(const HeadArgs& g, int dtype, int in_width, int out_width
     // rows of the result may not overlap; rows of the inputs may repeat (a stride of zero broadcasts)
     if (g.a_token < 0 || g.a_head < 0 || g.w_head < 0 || (g.heads > 1 && g.out_head < out_width) || (g.n_tokens > 1 && g.out_token < out_width))
         return VIB3_ERR_SHAPE;
-    (void)in_width;
     if (off16(g.a) || off16(g.w) || off16(g.out) || g.a_token % 8 || g.a_head % 8 || g.w_head % 8 || g.out_token % 8 || g.out_head % 8)
         return VIB3_ERR_ALIGN;
     return VIB3_OK;
@@ -429,7 +428,7 @@ extern "C" int vib3_launch_latent_query(const void* q, long long q_token_stride,
     HeadArgs g{q, q_token_stride, q_head_stride, w_uk, w_head_stride, out, out_token_stride, out_head_stride, n_tokens, heads, nope,
                positions, inv_freq, rope_scale, pairs, status};
     if ((n_tokens != 0 && !positions) || !inv_freq) return VIB3_ERR_NULL;
-    const int e = check_heads(g, dtype, nope + kRope, kLatentRow);
+    const int e = check_heads(g, dtype, kLatentRow);
     if (e) return e;
     if (n_tokens == 0) return VIB3_OK;
     return dtype == L_F16 ? launch_heads<__half, true>(g, dtype, (cudaStream_t)stream) : launch_heads<__nv_bfloat16, true>(g, dtype, (cudaStream_t)stream);
@@ -440,7 +439,7 @@ extern "C" int vib3_launch_latent_value(const void* o, long long o_token_stride,
                                         int n_tokens, int heads, int value, int dtype, int* status, void* stream) {
     HeadArgs g{o, o_token_stride, o_head_stride, w_uv, w_head_stride, out, out_token_stride, out_head_stride, n_tokens, heads, value,
                nullptr, nullptr, 1.f, 0, status};
-    const int e = check_heads(g, dtype, kRank, value);
+    const int e = check_heads(g, dtype, value);
     if (e) return e;
     if (n_tokens == 0) return VIB3_OK;
     return dtype == L_F16 ? launch_heads<__half, false>(g, dtype, (cudaStream_t)stream) : launch_heads<__nv_bfloat16, false>(g, dtype, (cudaStream_t)stream);

@@ -473,7 +473,8 @@ def latent_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Ten
     """Attention in the latent space over the paged cache (cuda/src/kernels.cu:1570 for the newest tokens of a batch): q [B * q_len,
     H, 576] (sequence b's q_len tokens together), cache [pages, page_size, 576], page_table [B, max_pages] int32, seq_lens [B] int32
     (keys of each sequence, its new tokens included) -> out [B * q_len, H, 512] and, if given, lse [B * q_len, H] fp32.  Token j of
-    a sequence sees the keys up to position seq_lens - q_len + j; a row that sees none is 0 and -inf.  ``workspace``: a uint8
+    a sequence sees the keys up to position seq_lens - q_len + j; a row that sees none is 0 and -inf.  Rows of the cache behind a length
+    may hold anything, those within it have to be finite.  ``workspace``: a uint8
     tensor of latent_attention_workspace_bytes(), not shared by calls that may overlap."""
     (T, H, width), (q0, q1, q2) = q.shape, q.stride()
     (pages, page, R), (c0, c1, c2) = cache.shape, cache.stride()
