@@ -6,6 +6,7 @@ import torch
 class Model:
     def __init__(self, hidden=64, n_layers=1):
         self.shape, self.n_layers = type("Shape", (), {"hidden": hidden, "num_experts": 6}), n_layers
+        self.router_w = torch.zeros(n_layers, 6, hidden)
 
 
 class Grouped:
@@ -123,3 +124,16 @@ def test_queries_of_low_rank_that_do_not_fit_are_refused_when_the_layer_is_made(
                    (z(160, 24), dict(q_down=z(24, 64), q_norm=z(23))), (z(160, 24), dict(q_down=z(24, 64), q_norm=z(24).float()))):
         with pytest.raises(ValueError):
             make(w_q, **k)
+
+
+def test_a_decoder_on_another_device_is_refused_when_the_layer_is_made(monkeypatch):
+    from vic_b200.attention import DecodeLayer
+    layer, _, _ = parts(monkeypatch, Grouped(128), 24, 12)
+    norm = torch.ones(64, dtype=torch.bfloat16)
+    elsewhere = Model()
+    elsewhere.router_w = torch.zeros(1, 6, 64, device="meta")
+    with pytest.raises(ValueError, match="moe"):
+        DecodeLayer(layer.attention, Grouped(128, elsewhere), 0, norm, norm)
+    for norms in ((norm.to("meta"), norm), (norm, norm.to("meta"))):
+        with pytest.raises(ValueError, match="norm"):
+            DecodeLayer(layer.attention, layer.moe, 0, *norms)

@@ -163,15 +163,15 @@ class DecodeLayer:
 
     def __init__(self, attention: LatentAttention, moe, layer: int, attention_norm: torch.Tensor, moe_norm: torch.Tensor, eps: float = 1e-6,
                  selection_bias: Optional[torch.Tensor] = None):
-        hidden = attention.shape.hidden
+        hidden, dev = attention.shape.hidden, attention.w_q.device
         for norm in (attention_norm, moe_norm):
-            if norm.shape != (hidden,) or norm.dtype not in (torch.float16, torch.bfloat16) or not norm.is_contiguous():
-                raise ValueError(f"norm weights: contiguous fp16 or bf16 [{hidden}] expected")
-        if moe.model.shape.hidden != hidden or not -moe.model.n_layers <= layer < moe.model.n_layers:
-            raise ValueError(f"moe: a decoder with layer {layer} and rows of {hidden} values expected")
+            if norm.shape != (hidden,) or norm.dtype not in (torch.float16, torch.bfloat16) or not norm.is_contiguous() or norm.device != dev:
+                raise ValueError(f"norm weights: contiguous fp16 or bf16 [{hidden}] on {dev} expected")
+        if moe.model.shape.hidden != hidden or not -moe.model.n_layers <= layer < moe.model.n_layers or moe.model.router_w.device != dev:
+            raise ValueError(f"moe: a decoder on {dev} with layer {layer} and rows of {hidden} values expected")
         if selection_bias is not None and (selection_bias.shape != (moe.model.shape.num_experts,) or selection_bias.dtype != torch.float32
-                                           or not selection_bias.is_contiguous() or selection_bias.device != attention.w_q.device):
-            raise ValueError(f"selection_bias: contiguous fp32 [{moe.model.shape.num_experts}] on {attention.w_q.device} expected")
+                                           or not selection_bias.is_contiguous() or selection_bias.device != dev):
+            raise ValueError(f"selection_bias: contiguous fp32 [{moe.model.shape.num_experts}] on {dev} expected")
         self.selection_bias = selection_bias
         self.attention, self.moe, self.layer = attention, moe, layer
         self.moe_rows = getattr(moe, "max_tokens", 1)       # of a GroupedDecoder; a MoeDecoder takes one row
