@@ -102,41 +102,54 @@ def rms_norm_f32(input_f32, output_f32, weight_f16, hidden_dim: int, eps: float,
 EXACT_HOLD = 2   # added to a router launch's exact_order: the producer of x lets its dependents start early
 
 
-def _holds_rows(t: torch.Tensor, T: int, H: int) -> bool:
-    """Whether t has T rows of H contiguous values (a single row may be a vector)."""
-    if t.dim() == 1:
-        return T <= 1 and t.shape[0] >= H and t.stride(0) == 1
-    return t.dim() == 2 and t.shape[0] >= T and t.shape[1] >= H and t.stride(1) == 1
+_X_TYPES = {torch.float32: (X_F32, 4), torch.float16: (X_F16, 2), torch.bfloat16: (X_BF16, 2)}     # code, bytes
+
+
+def _row_stride(t: torch.Tensor, shape) -> Optional[int]:
+    """From row to row of t, if it has a contiguous row for each of [T, H] (a single one may be a vector); None otherwise."""
+    if t.shape == shape or (t.dim() == 2 and t.shape[0] >= shape[0] and t.shape[1] >= shape[1]):
+        stride, last = t.stride()
+        return stride if last == 1 else None
+    return 1 if t.dim() == 1 and shape[0] <= 1 and t.shape[0] >= shape[1] and t.stride(0) == 1 else None
 
 
 def residual_rms_norm(hidden: torch.Tensor, delta, weight_f16, eps: float, x_out: torch.Tensor, stream: Optional[int] = None,
                       delta2=None, center: bool = False, early_dependents: bool = False) -> None:
     """hidden [T, H] fp32 += delta [T, H] + delta2 [T, H] fp32 (either may be None); x_out [T, H] = cast(rms_norm(hidden) *
-    weight) with ``weight_f16`` [H] fp16 or, as a tensor of that type, bf16 (None: no weight): one launch.  ``early_dependents``: the next launch of the stream may start while this one runs; it must
-    be a router launch with ``EXACT_HOLD`` added to its exact_order argument (see include/vib3_b200.h)."""
-    if hidden.dim() != 2 or hidden.dtype != torch.float32 or hidden.stride(1) != 1:
+    weight) with ``weight_f16`` [H] fp16 or, as a tensor of that type, bf16 (None: no weight): one launch.
+    ``early_dependents``: the next launch of the stream may start while this one runs; it must be a router launch with ``EXACT_HOLD`` added to its exact_order argument (see include/vib3_b200.h)."""
+    shape = hidden.shape
+    if len(shape) != 2 or hidden.dtype != torch.float32 or hidden.stride(1) != 1:
         raise ValueError("hidden: fp32 [T, H] with contiguous rows expected")
-    T, H = hidden.shape
     # (the launcher knows addresses and strides only: what is smaller than hidden would be written or read behind its end)
-    if x_out.dtype not in _X_CODES or not _holds_rows(x_out, T, H) or (T > 1 and x_out.stride(0) < H):
+    T, H = shape
+    x_type, x_stride = _X_TYPES.get(x_out.dtype), _row_stride(x_out, shape)
+    if x_type is None or x_stride is None or (T > 1 and x_stride < H):
         raise ValueError("x_out: fp32, fp16 or bf16 with room for hidden's rows, each contiguous, expected")
-    if delta is not None and (delta.dtype not in _X_CODES or not _holds_rows(delta, T, H)):
-        raise ValueError("delta: fp32, fp16 or bf16 with a contiguous row for each of hidden's expected")
-    if delta2 is not None and (delta2.dtype != torch.float32 or not _holds_rows(delta2, T, H)):
-        raise ValueError("delta2: fp32 with a contiguous row for each of hidden's expected")
+    d_type, d_stride = (0, 0), 0
+    if delta is not None:
+        d_type, d_stride = _X_TYPES.get(delta.dtype), _row_stride(delta, shape)
+        if d_type is None or d_stride is None:
+            raise ValueError("delta: fp32, fp16 or bf16 with a contiguous row for each of hidden's expected")
+    d2_stride = 0
+    if delta2 is not None:
+        d2_stride = _row_stride(delta2, shape)
+        if delta2.dtype != torch.float32 or d2_stride is None:
+            raise ValueError("delta2: fp32 with a contiguous row for each of hidden's expected")
     flags = int(center) | (2 if early_dependents else 0)
     if isinstance(weight_f16, torch.Tensor):
-        if weight_f16.dtype == torch.bfloat16:
+        w_type = weight_f16.dtype
+        if w_type == torch.bfloat16:
             flags |= 4
-        elif weight_f16.dtype != torch.float16:
-            raise ValueError(f"norm weights: fp16 or bf16 expected, got {weight_f16.dtype}")
+        elif w_type != torch.float16:
+            raise ValueError(f"norm weights: fp16 or bf16 expected, got {w_type}")
         if weight_f16.numel() < H or not weight_f16.is_contiguous():
             raise ValueError("norm weights: contiguous [H] expected")
-    check("residual_rms_norm", lib().vib3_launch_residual_rms_norm(
-        _ptr(hidden), hidden.stride(0), _ptr(delta), x_dtype_code(delta) if delta is not None else 0,
-        delta.stride(0) * delta.element_size() if delta is not None else 0, _ptr(delta2),
-        delta2.stride(0) if delta2 is not None else 0, _ptr(weight_f16), eps, flags, _ptr(x_out),
-        x_dtype_code(x_out), x_out.stride(0) * x_out.element_size(), H, T, _stream(stream)))
+    err = lib().vib3_launch_residual_rms_norm(
+        _ptr(hidden), hidden.stride(0), _ptr(delta), d_type[0], d_stride * d_type[1], _ptr(delta2), d2_stride, _ptr(weight_f16), eps, flags,
+        _ptr(x_out), x_type[0], x_stride * x_type[1], H, T, _stream(stream))
+    if err:
+        check("residual_rms_norm", err)
 
 
 def router_gemv_f32(hidden_state, router_weights_f16, scores, hidden_dim: int, num_experts: int,
