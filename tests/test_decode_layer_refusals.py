@@ -121,7 +121,8 @@ def test_queries_of_low_rank_that_do_not_fit_are_refused_when_the_layer_is_made(
     make(z(160, 24), q_down=z(24, 64), q_norm=z(24))
     for w_q, k in ((z(160, 24), {}), (z(160, 64), dict(q_down=z(24, 64), q_norm=z(24))), (z(160, 24), dict(q_down=z(24, 64))), (z(160, 64), dict(q_norm=z(64))),
                    (z(160, 24), dict(q_down=z(24, 32), q_norm=z(24))), (z(160, 24), dict(q_down=z(24, 64).half(), q_norm=z(24))),
-                   (z(160, 24), dict(q_down=z(24, 64), q_norm=z(23))), (z(160, 24), dict(q_down=z(24, 64), q_norm=z(24).float()))):
+                   (z(160, 24), dict(q_down=z(24, 64), q_norm=z(23))), (z(160, 24), dict(q_down=z(24, 64), q_norm=z(24).float())),
+                   (z(160, 24), dict(q_down=z(24, 64), q_norm=z(24).to("meta"))), (z(160, 24), dict(q_down=z(24, 64).to("meta"), q_norm=z(24)))):
         with pytest.raises(ValueError):
             make(w_q, **k)
 

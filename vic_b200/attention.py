@@ -101,11 +101,11 @@ class LatentAttention:
             raise ValueError("q_down and q_norm: both or neither")
         q_width = shape.hidden
         if q_down is not None:
-            if q_down.dim() != 2 or q_down.shape[1] != shape.hidden or q_down.dtype != dt:
-                raise ValueError(f"q_down: [q_rank, {shape.hidden}] of the layer's dtype expected")
+            if q_down.dim() != 2 or q_down.shape[1] != shape.hidden or q_down.dtype != dt or q_down.device != dev:
+                raise ValueError(f"q_down: [q_rank, {shape.hidden}] of the layer's dtype on {dev} expected")
             q_width = q_down.shape[0]
-            if q_norm.shape != (q_width,) or q_norm.dtype not in (torch.float16, torch.bfloat16) or not q_norm.is_contiguous():
-                raise ValueError(f"q_norm: contiguous fp16 or bf16 [{q_width}] expected")
+            if q_norm.shape != (q_width,) or q_norm.dtype not in (torch.float16, torch.bfloat16) or not q_norm.is_contiguous() or q_norm.device != dev:
+                raise ValueError(f"q_norm: contiguous fp16 or bf16 [{q_width}] on {dev} expected")
             self.q_low32 = torch.zeros(max_tokens, q_width, device=dev)
             self.q_low = torch.zeros(max_tokens, q_width, dtype=dt, device=dev)
         self.q_down, self.q_norm = q_down, q_norm
