@@ -41,3 +41,13 @@ def test_larger_buffers_and_single_rows_pass_the_comparison(change):
     """What is refused here is the device: every operand lies on the CPU."""
     with pytest.raises(ValueError, match="device tensor"):
         norm(**change)
+
+
+@pytest.mark.gpu
+def test_a_hidden_state_on_another_device_than_the_current_one(cuda_dev, monkeypatch):
+    from vic_b200 import kernels
+    a = {n: torch.zeros(3, 64, device=cuda_dev) for n in ("hidden", "x_out")}
+    norm(**a, weight_f16=None)
+    monkeypatch.setattr(kernels, "_current_device", lambda: 1)
+    with pytest.raises(ValueError, match="current device"):
+        norm(**a, weight_f16=None)

@@ -121,6 +121,8 @@ def residual_rms_norm(hidden: torch.Tensor, delta, weight_f16, eps: float, x_out
     shape = hidden.shape
     if len(shape) != 2 or hidden.dtype != torch.float32 or hidden.stride(1) != 1:
         raise ValueError("hidden: fp32 [T, H] with contiguous rows expected")
+    if hidden.is_cuda and hidden.get_device() != _current_device():     # (a launch on another one would read through a foreign context)
+        raise ValueError(f"hidden: on the current device (cuda:{_current_device()}) expected, got {hidden.device}")
     # (the launcher knows addresses and strides only: what is smaller than hidden would be written or read behind its end)
     T, H = shape
     x_type, x_stride = _X_TYPES.get(x_out.dtype), _row_stride(x_out, shape)
